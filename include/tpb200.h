@@ -400,6 +400,47 @@ int tp_b200_gemm_epilogue(int epilogue, const tpb_tensor* out, const tpb_tensor*
                           double alpha, double beta, int flags, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Feed-forward blocks (no single counterpart in the reference: sequences of
+ * linear (BlasKernels.cpp:374-386), the activations of UnaryKernels.cpp:52-104
+ * and mul / add (BinaryKernels.cpp:148-248)).  bfloat16, float16 and float32.
+ * "Gated" tensors are [rows, 2, n], the gate's part first.
+ *
+ * 8-bit checkpoints keep an activation's input for the backward pass: every
+ * block of 32 consecutive elements of a row is int8 values q and one uint8
+ * exponent s, standing for q * 2^(s - 127): the least power of two with
+ * max|x| <= 127 * 2^(s - 127), x / 2^(s - 127) rounded to the nearest
+ * integer, ties to even.  s = 255 marks a block that held an infinity or a
+ * NaN and reads back as NaN.  values has the tensor's shape, exponents
+ * ceil(n / 32) in the last dimension; both contiguous.
+ * ---------------------------------------------------------------------- */
+
+enum tpb_activation {
+    TPB_ACT_NONE = 0,
+    TPB_ACT_RELU = 1,
+    TPB_ACT_GELU = 2,      /* exact (normal CDF) form */
+    TPB_ACT_GELU_TANH = 3, /* approximate="tanh"      */
+    TPB_ACT_SILU = 4
+};
+
+/* y = act(z) [+ residual] for z [rows, n], y = act(z0) * z1 [+ residual] for
+ * z [rows, 2, n]; y [rows, n] may be NULL.  values / exponents (may be NULL)
+ * receive the checkpoint of z.  Rows may be strided; computed in fp32 and
+ * rounded once. */
+int tp_b200_activation_forward(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
+                               const tpb_tensor* z, const tpb_tensor* residual, int act, void* stream);
+/* The gradient of activation_forward's z (shaped like dz): dz = dy * act'(z),
+ * or dz0 = dy * z1 * act'(z0) and dz1 = dy * act(z0).  z is a tensor, or NULL
+ * and given as a checkpoint.  partial (may be NULL): fp32 [b, parts * n],
+ * 1 <= b <= 65535, receives the column sums of dz over b groups of rows,
+ * taken before dz is rounded (their sum is the bias gradient). */
+int tp_b200_activation_backward(const tpb_tensor* dz, const tpb_tensor* partial, const tpb_tensor* dy,
+                                const tpb_tensor* z, const tpb_tensor* values, const tpb_tensor* exponents, int act,
+                                void* stream);
+/* y [rows, n] = what a checkpoint stands for, rounded to y's dtype. */
+int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
+                              void* stream);
+
+/* ------------------------------------------------------------------------
  * Collectives over NCCL (replaces tensorplay_mlu/csrc/Cncl.cpp:71-387; same
  * argument order, codes and status convention).  Each collective is ordered
  * on the calling thread's current stream of `dev` (tp_b200_set_stream).

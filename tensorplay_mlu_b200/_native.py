@@ -43,6 +43,9 @@ ADD, SUB, MUL, DIV, RSUB = range(5)
 SUM, MEAN, AMAX, AMIN = range(4)
 EPI_GELU, EPI_GELU_BACKWARD = 1, 2  # tp_b200_gemm_epilogue
 GEMM_ALLOW_TF32 = 1
+# tpb_activation
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+CHECKPOINT_BLOCK = 32  # elements that share one checkpoint exponent
 
 
 class TpbTensor(ctypes.Structure):
@@ -140,6 +143,9 @@ _SIGNATURES = {
     "tp_b200_nll_loss_backward": ([_T, _T, _T, _T, _T, _I, _I64, _P], _I),
     "tp_b200_dropout": ([_T, _T, _T, _D, ctypes.c_uint64, ctypes.c_uint64, _P], _I),
     "tp_b200_masked_scale": ([_T, _T, _T, _D, _P], _I),
+    "tp_b200_activation_forward": ([_T, _T, _T, _T, _T, _I, _P], _I),
+    "tp_b200_activation_backward": ([_T, _T, _T, _T, _T, _T, _I, _P], _I),
+    "tp_b200_checkpoint_unpack": ([_T, _T, _T, _P], _I),
     "tp_b200_nccl_last_error": ([], ctypes.c_char_p),
     "tp_b200_nccl_unique_id_bytes": ([], _I),
     "tp_b200_nccl_get_unique_id": ([_P], _I),

@@ -1,0 +1,603 @@
+// Elementwise kernels of the feed-forward operators: the activation, gate and
+// residual behind a product (where the product's own epilogue does not apply
+// them), their backward pass with the bias gradient, and 8-bit checkpoints.
+//
+// tensorplay-mlu runs these as separate activation, mul and add kernels
+// (UnaryKernels.cpp:52-104, BinaryKernels.cpp:148-248) and has no
+// checkpoints.  All are bound by memory: each reads its inputs and writes its
+// results once.
+
+#include "act.cuh"
+
+namespace tpb {
+namespace {
+
+// V consecutive elements of a row as floats: 16-byte loads for V = 8 (one for
+// 16-bit types, two for fp32), one element for V = 1.
+template <typename T, int V>
+struct RowVec {
+    static constexpr int kPer = V == 1 ? 1 : (16 / int(sizeof(T)) < V ? 16 / int(sizeof(T)) : V);
+    Vec<T, kPer> part[V / kPer];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < V / kPer; ++i) part[i] = reinterpret_cast<const Vec<T, kPer>*>(p)[i];
+    }
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V / kPer; ++i) {
+            float t[kPer];
+            unpack_vec(part[i], t);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) f[i * kPer + j] = t[j];
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[V]) {
+#pragma unroll
+        for (int i = 0; i < V / kPer; ++i) {
+            float t[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) t[j] = f[i * kPer + j];
+            pack_vec(t, part[i]);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int i = 0; i < V / kPer; ++i) reinterpret_cast<Vec<T, kPer>*>(p)[i] = part[i];
+    }
+};
+
+// Rows of 32-element blocks: unit u is block u % nb of row u / nb, and 32 / V
+// neighbouring lanes share it.
+struct Units {
+    int64_t count;
+    int64_t nb;
+    FastDiv div;
+    __device__ __forceinline__ void split(int64_t u, int64_t& row, int64_t& blk) const {
+        row = count <= 0xffffffffll ? int64_t(div.div(uint32_t(u))) : u / nb;
+        blk = u - row * nb;
+    }
+};
+
+Units make_units(int64_t rows, int64_t n) {
+    Units u;
+    u.nb = (n + kCkptBlock - 1) / kCkptBlock;
+    u.count = rows * u.nb;
+    u.div = FastDiv(static_cast<uint32_t>(std::min<int64_t>(u.nb, 0xffffffffll)));
+    return u;
+}
+
+// One block's values and exponent, from V elements in each of its lanes.
+template <typename T, int V>
+__device__ __forceinline__ void pack_block(const float (&x)[V], int count, int lane_in_block, int8_t* values,
+                                           uint8_t* exponent) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) amax = max_nan(amax, fabsf(x[j]));
+#pragma unroll
+    for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float qmax;
+    const int stored = ckpt_exponent<T>(amax, qmax);
+    const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+    Vec<int8_t, V> q;
+#pragma unroll
+    for (int j = 0; j < V; ++j) q.v[j] = ckpt_quantise(x[j], inverse, qmax);
+    if (count == V) *reinterpret_cast<Vec<int8_t, V>*>(values) = q;
+    if (lane_in_block == 0 && exponent != nullptr) *exponent = static_cast<uint8_t>(stored);
+}
+
+template <typename T>
+struct ForwardParams {
+    const T* z;
+    int64_t sz_m, sz_p;
+    const T* residual;
+    int64_t sr_m;
+    T* y;
+    int64_t sy_m;
+    int8_t* values;     // [rows, parts, n], contiguous
+    uint8_t* exponents; // [rows, parts, nb], contiguous
+    int64_t n;
+    int act;
+    Units units;
+};
+
+// y = act(z0) [* z1] [+ residual] and the checkpoint of z0 [and z1]; a thread
+// holds V elements of a unit, kU units at a time so that their loads are in
+// flight together.
+template <typename T, int V, bool GATED>
+__global__ void __launch_bounds__(kThreads) ffn_forward_kernel(const ForwardParams<T> p) {
+    pdl_entry();
+    constexpr int kLanes = kCkptBlock / V;
+    constexpr int kU = V == 1 ? 8 : 4;
+    constexpr int kParts = GATED ? 2 : 1;
+    constexpr bool kFast = Narrow<T>::value;
+    const int lane = threadIdx.x % kLanes;
+    const int64_t per_pass = int64_t(blockDim.x / kLanes);
+    int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
+    RowVec<T, V> in[kU][kParts], res[kU];
+    int64_t row[kU], blk[kU];
+    bool ok[kU];
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+        const int64_t u = u0 + i * per_pass;
+        ok[i] = u < p.units.count;
+        if (!ok[i]) continue;
+        p.units.split(u, row[i], blk[i]);
+        const int64_t col = blk[i] * kCkptBlock + lane * V;
+        ok[i] = col < p.n;
+        if (!ok[i]) continue;
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) in[i][q].load(p.z + row[i] * p.sz_m + q * p.sz_p + col);
+        if (p.residual != nullptr) res[i].load(p.residual + row[i] * p.sr_m + col);
+    }
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+        const int64_t u = u0 + i * per_pass;
+        const int64_t col = blk[i] * kCkptBlock + lane * V;
+        float z[kParts][V];
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+            if (ok[i]) in[i][q].get(z[q]);
+            else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) z[q][j] = 0.0f;
+            }
+        }
+        if (p.values != nullptr) {
+#pragma unroll
+            for (int q = 0; q < kParts; ++q) {
+                const bool in_range = u < p.units.count;
+                const int64_t at = in_range ? row[i] * kParts + q : 0;
+                pack_block<T, V>(z[q], ok[i] ? V : 0, lane, p.values + at * p.n + (ok[i] ? col : 0),
+                                 in_range ? p.exponents + at * p.units.nb + blk[i] : nullptr);
+            }
+        }
+        if (p.y != nullptr && ok[i]) {
+            act_values<kFast, V>(p.act, z[0]);
+            if constexpr (GATED) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) z[0][j] *= z[1][j];
+            }
+            if (p.residual != nullptr) {
+                float r[V];
+                res[i].get(r);
+#pragma unroll
+                for (int j = 0; j < V; ++j) z[0][j] += r[j];
+            }
+            RowVec<T, V> out;
+            out.set(z[0]);
+            out.store(p.y + row[i] * p.sy_m + col);
+        }
+    }
+}
+
+template <typename T>
+struct UnpackParams {
+    T* y;
+    int64_t sy_m;
+    const int8_t* values;
+    const uint8_t* exponents;
+    int64_t n;
+    Units units;
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const UnpackParams<T> p) {
+    pdl_entry();
+    constexpr int kLanes = kCkptBlock / V;
+    constexpr int kU = 4;
+    const int lane = threadIdx.x % kLanes;
+    const int64_t per_pass = int64_t(blockDim.x / kLanes);
+    const int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
+    Vec<int8_t, V> q[kU];
+    int stored[kU];
+    int64_t row[kU], col[kU];
+    bool ok[kU];
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+        const int64_t u = u0 + i * per_pass;
+        ok[i] = u < p.units.count;
+        if (!ok[i]) continue;
+        int64_t blk;
+        p.units.split(u, row[i], blk);
+        col[i] = blk * kCkptBlock + lane * V;
+        ok[i] = col[i] < p.n;
+        if (!ok[i]) continue;
+        q[i] = *reinterpret_cast<const Vec<int8_t, V>*>(p.values + row[i] * p.n + col[i]);
+        stored[i] = p.exponents[u];
+    }
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+        if (!ok[i]) continue;
+        const float step = ckpt_step(stored[i]);
+        float f[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = float(q[i].v[j]) * step;
+        RowVec<T, V> out;
+        out.set(f);
+        out.store(p.y + row[i] * p.sy_m + col[i]);
+    }
+}
+
+template <typename T>
+struct BackwardParams {
+    const T* dy;
+    int64_t sdy_m;
+    const T* z;
+    int64_t sz_m, sz_p;
+    const int8_t* values;
+    const uint8_t* exponents;
+    int64_t nb;
+    T* dz;
+    int64_t sdz_m, sdz_p;
+    float* partial;  // [gridDim.y, parts, n] column sums of dz, or null
+    int64_t m, n;
+    int64_t rows_per_block;
+    int act;
+    int tx;  // threads along the columns (a power of two)
+};
+
+// dz0 = dy [* z1] act'(z0) [, dz1 = dy act(z0)] and, for the bias gradient,
+// the fp32 sums of dz (before its rounding) over the block's rows.  A thread
+// keeps its V columns and walks the rows, so the sums stay in registers; they
+// are joined over the block in a fixed order and written as one partial row.
+template <typename T, int V, bool GATED, bool SAVED8>
+__global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardParams<T> p) {
+    pdl_entry();
+    constexpr int kParts = GATED ? 2 : 1;
+    constexpr int kU = GATED ? 2 : 4;
+    constexpr bool kFast = Narrow<T>::value;
+    const int tx = threadIdx.x & (p.tx - 1);
+    const int ty = threadIdx.x / p.tx;
+    const int ny = kThreads / p.tx;
+    const int64_t col = (int64_t(blockIdx.x) * p.tx + tx) * V;
+    const int64_t r1 = min(p.m, (int64_t(blockIdx.y) + 1) * p.rows_per_block);
+    const bool col_ok = col < p.n;
+    float acc[kParts][V];
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[q][j] = 0.0f;
+    }
+    if (col_ok) {
+        for (int64_t r = int64_t(blockIdx.y) * p.rows_per_block + ty; r < r1; r += int64_t(ny) * kU) {
+            RowVec<T, V> dyv[kU], zv[kU][kParts];
+            Vec<int8_t, V> qv[kU][kParts];
+            int ev[kU][kParts];
+#pragma unroll
+            for (int i = 0; i < kU; ++i) {
+                const int64_t row = r + int64_t(i) * ny;
+                if (row >= r1) continue;
+                dyv[i].load(p.dy + row * p.sdy_m + col);
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    if constexpr (SAVED8) {
+                        const int64_t at = row * kParts + q;
+                        qv[i][q] = *reinterpret_cast<const Vec<int8_t, V>*>(p.values + at * p.n + col);
+                        ev[i][q] = p.exponents[at * p.nb + col / kCkptBlock];
+                    } else {
+                        zv[i][q].load(p.z + row * p.sz_m + q * p.sz_p + col);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kU; ++i) {
+                const int64_t row = r + int64_t(i) * ny;
+                if (row >= r1) continue;
+                float dy[V], z[kParts][V], a[V], d[V];
+                dyv[i].get(dy);
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    if constexpr (SAVED8) {
+                        const float step = ckpt_step(ev[i][q]);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) z[q][j] = float(qv[i][q].v[j]) * step;
+                    } else {
+                        zv[i][q].get(z[q]);
+                    }
+                }
+                act_slopes<kFast, V>(p.act, z[0], a, d);
+                RowVec<T, V> out;
+                if constexpr (GATED) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        a[j] *= dy[j];
+                        acc[1][j] += a[j];
+                        dy[j] *= z[1][j];
+                    }
+                    out.set(a);
+                    out.store(p.dz + row * p.sdz_m + p.sdz_p + col);
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    d[j] *= dy[j];
+                    acc[0][j] += d[j];
+                }
+                out.set(d);
+                out.store(p.dz + row * p.sdz_m + col);
+            }
+        }
+    }
+    if (p.partial == nullptr) return;
+    __shared__ float sums[kThreads * V];
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) sums[j * kThreads + threadIdx.x] = acc[q][j];
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.tx * V; c += kThreads) {
+            const int x = c / V, j = c % V;
+            const int64_t at = (int64_t(blockIdx.x) * p.tx + x) * V + j;
+            if (at >= p.n) continue;
+            float s = 0.0f;
+            for (int y = 0; y < ny; ++y) s += sums[j * kThreads + y * p.tx + x];
+            p.partial[(int64_t(blockIdx.y) * kParts + q) * p.n + at] = s;
+        }
+    }
+}
+
+void require_dtype(const tpb_tensor& t, int dtype, const char* what) {
+    TPB_CHECK(t.dtype == dtype, "%s: expected %s, got %s", what, dtype_name(dtype), dtype_name(t.dtype));
+}
+
+void require_act(int act, const char* what) {
+    TPB_CHECK(act >= TPB_ACT_NONE && act <= TPB_ACT_SILU, "%s: unknown activation %d", what, act);
+}
+
+void require_float(const tpb_tensor& t, const char* what) {
+    TPB_CHECK(t.dtype == TPB_BF16 || t.dtype == TPB_F16 || t.dtype == TPB_F32,
+              "%s: expected bfloat16, float16 or float32, got %s", what, dtype_name(t.dtype));
+}
+
+// [rows, n] or [rows, 2, n] with unit stride along n.
+void require_rows(const tpb_tensor& t, const char* what) {
+    TPB_CHECK(t.ndim == 2 || (t.ndim == 3 && t.sizes[1] == 2), "%s: expected [rows, n] or [rows, 2, n]", what);
+    TPB_CHECK(t.strides[t.ndim - 1] == 1 || t.sizes[t.ndim - 1] <= 1, "%s: needs unit stride along its last dimension",
+              what);
+}
+
+void require_same(const tpb_tensor& a, const tpb_tensor& b, const char* what) {
+    TPB_CHECK(a.ndim == b.ndim, "%s: rank mismatch (%d vs %d)", what, a.ndim, b.ndim);
+    for (int i = 0; i < a.ndim; ++i) {
+        TPB_CHECK(a.sizes[i] == b.sizes[i], "%s: size mismatch at dimension %d (%lld vs %lld)", what, i,
+                  (long long)a.sizes[i], (long long)b.sizes[i]);
+    }
+}
+
+// int8 values shaped like `z` and uint8 exponents [.., ceil(n / 32)], dense.
+void require_checkpoint(const tpb_tensor* values, const tpb_tensor* exponents, const tpb_tensor& z, const char* what) {
+    check_tensor(values, what);
+    check_tensor(exponents, what);
+    require_dtype(*values, TPB_I8, what);
+    require_dtype(*exponents, TPB_U8, what);
+    require_same(*values, z, what);
+    TPB_CHECK(is_contiguous(*values) && is_contiguous(*exponents), "%s: checkpoints are contiguous", what);
+    TPB_CHECK(exponents->ndim == z.ndim, "%s: exponents need the values' rank", what);
+    for (int i = 0; i < z.ndim; ++i) {
+        const int64_t want = i == z.ndim - 1 ? (z.sizes[i] + kCkptBlock - 1) / kCkptBlock : z.sizes[i];
+        TPB_CHECK(exponents->sizes[i] == want, "%s: exponents have %lld, not %lld, at dimension %d", what,
+                  (long long)exponents->sizes[i], (long long)want, i);
+    }
+}
+
+// 16-byte vectors along n are possible for an operand of `es`-byte elements.
+bool rows16(const void* p, int64_t pitch, size_t es) {
+    return p == nullptr || (aligned16(p) && (pitch * int64_t(es)) % 16 == 0);
+}
+
+unsigned unit_blocks(const Units& u, int lanes, int unroll) {
+    const int64_t blocks = (u.count + int64_t(kThreads / lanes) * unroll - 1) / (int64_t(kThreads / lanes) * unroll);
+    TPB_CHECK(blocks < (int64_t(1) << 31), "checkpoint: too many elements for one call");
+    return static_cast<unsigned>(blocks);
+}
+
+template <typename T, bool GATED>
+void launch_forward(ForwardParams<T>& p, cudaStream_t s) {
+    const bool vec = p.n % 8 == 0 && rows16(p.z, p.sz_m, sizeof(T)) && rows16(p.z, p.sz_p, sizeof(T)) &&
+                     rows16(p.residual, p.sr_m, sizeof(T)) && rows16(p.y, p.sy_m, sizeof(T)) &&
+                     reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    if (vec) {
+        launch_pdl(ffn_forward_kernel<T, 8, GATED>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
+    } else {
+        launch_pdl(ffn_forward_kernel<T, 1, GATED>, unit_blocks(p.units, 32, 8), kThreads, 0, s, p);
+    }
+    check_launch("ffn_forward");
+}
+
+template <typename T, int V, bool GATED, bool SAVED8>
+void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaStream_t s) {
+    // Threads along the columns: enough for one row, at most the block.
+    int tx = 1;
+    while (tx < kThreads && int64_t(tx) * V < p.n) tx <<= 1;
+    p.tx = tx;
+    const int64_t gx = (p.n + int64_t(tx) * V - 1) / (int64_t(tx) * V);
+    int64_t gy;
+    if (p.partial != nullptr) {
+        gy = partial_rows;
+    } else {
+        // About eight blocks an SM, and no more than one pass of rows needs.
+        const int64_t pass = int64_t(kThreads / tx) * (GATED ? 2 : 4);
+        gy = std::max<int64_t>(1, std::min<int64_t>((p.m + pass - 1) / pass, (int64_t(num_sms(dev)) * 8 + gx - 1) / gx));
+        gy = std::min<int64_t>(gy, 65535);
+    }
+    p.rows_per_block = (p.m + gy - 1) / gy;
+    TPB_CHECK(gx < (int64_t(1) << 31), "activation_backward: too many columns");
+    launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8>, dim3(unsigned(gx), unsigned(gy)), kThreads, 0, s, p);
+    check_launch("ffn_backward");
+}
+
+template <typename T, bool GATED>
+void dispatch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaStream_t s) {
+    const bool vec = p.n % 8 == 0 && rows16(p.dy, p.sdy_m, sizeof(T)) && rows16(p.z, p.sz_m, sizeof(T)) &&
+                     rows16(p.z, p.sz_p, sizeof(T)) && rows16(p.dz, p.sdz_m, sizeof(T)) &&
+                     rows16(p.dz, p.sdz_p, sizeof(T)) && reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    if (p.values != nullptr) {
+        if (vec) launch_backward<T, 8, GATED, true>(p, partial_rows, dev, s);
+        else launch_backward<T, 1, GATED, true>(p, partial_rows, dev, s);
+    } else {
+        if (vec) launch_backward<T, 8, GATED, false>(p, partial_rows, dev, s);
+        else launch_backward<T, 1, GATED, false>(p, partial_rows, dev, s);
+    }
+}
+
+#define TPB_DISPATCH_FFN(dtype, what, ...)                                        \
+    switch (dtype) {                                                              \
+        case TPB_F16: { using scalar_t = __half; __VA_ARGS__; break; }            \
+        case TPB_F32: { using scalar_t = float; __VA_ARGS__; break; }             \
+        case TPB_BF16: { using scalar_t = __nv_bfloat16; __VA_ARGS__; break; }    \
+        default: TPB_CHECK(false, "%s: unsupported dtype %s", what, dtype_name(dtype)); \
+    }
+
+}  // namespace
+}  // namespace tpb
+
+using namespace tpb;
+
+extern "C" {
+
+int tp_b200_activation_forward(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
+                               const tpb_tensor* z, const tpb_tensor* residual, int act, void* stream) {
+    return guarded([&] {
+        check_tensor(z, "activation_forward z");
+        require_float(*z, "activation_forward z");
+        require_rows(*z, "activation_forward z");
+        require_act(act, "activation_forward");
+        const bool gated = z->ndim == 3;
+        const int64_t m = z->sizes[0], n = z->sizes[z->ndim - 1];
+        for (const tpb_tensor* t : {y, residual}) {
+            if (t == nullptr) continue;
+            check_tensor(t, "activation_forward result or residual");
+            require_dtype(*t, z->dtype, "activation_forward result or residual");
+            require_rows(*t, "activation_forward result or residual");
+            TPB_CHECK(t->ndim == 2 && t->sizes[0] == m && t->sizes[1] == n,
+                      "activation_forward: result and residual are [%lld, %lld]", (long long)m, (long long)n);
+        }
+        TPB_CHECK((values == nullptr) == (exponents == nullptr), "activation_forward: a checkpoint is values and exponents");
+        TPB_CHECK(y != nullptr || values != nullptr, "activation_forward: nothing to compute");
+        if (values != nullptr) require_checkpoint(values, exponents, *z, "activation_forward checkpoint");
+        if (m == 0 || n == 0) return;
+        const int dev = device_of(z->data);
+        DeviceGuard guard(dev);
+        cudaStream_t s = resolve_stream(stream, dev);
+        TPB_DISPATCH_FFN(z->dtype, "activation_forward", {
+            ForwardParams<scalar_t> p{};
+            p.z = static_cast<const scalar_t*>(z->data);
+            p.sz_m = z->strides[0];
+            p.sz_p = gated ? z->strides[1] : 0;
+            if (residual != nullptr) {
+                p.residual = static_cast<const scalar_t*>(residual->data);
+                p.sr_m = residual->strides[0];
+            }
+            if (y != nullptr) {
+                p.y = static_cast<scalar_t*>(y->data);
+                p.sy_m = y->strides[0];
+            }
+            if (values != nullptr) {
+                p.values = static_cast<int8_t*>(values->data);
+                p.exponents = static_cast<uint8_t*>(exponents->data);
+            }
+            p.n = n;
+            p.act = act;
+            p.units = make_units(m, n);
+            if (gated) launch_forward<scalar_t, true>(p, s);
+            else launch_forward<scalar_t, false>(p, s);
+        });
+    });
+}
+
+int tp_b200_activation_backward(const tpb_tensor* dz, const tpb_tensor* partial, const tpb_tensor* dy,
+                                const tpb_tensor* z, const tpb_tensor* values, const tpb_tensor* exponents, int act,
+                                void* stream) {
+    return guarded([&] {
+        check_tensor(dz, "activation_backward dz");
+        check_tensor(dy, "activation_backward dy");
+        require_float(*dz, "activation_backward dz");
+        require_dtype(*dy, dz->dtype, "activation_backward dy");
+        require_rows(*dz, "activation_backward dz");
+        require_rows(*dy, "activation_backward dy");
+        require_act(act, "activation_backward");
+        const bool gated = dz->ndim == 3;
+        const int64_t m = dz->sizes[0], n = dz->sizes[dz->ndim - 1];
+        TPB_CHECK(dy->ndim == 2 && dy->sizes[0] == m && dy->sizes[1] == n, "activation_backward: dy is [%lld, %lld]",
+                  (long long)m, (long long)n);
+        TPB_CHECK((z == nullptr) != (values == nullptr),
+                  "activation_backward: the activation's input is given as a tensor or as a checkpoint");
+        if (z != nullptr) {
+            check_tensor(z, "activation_backward z");
+            require_dtype(*z, dz->dtype, "activation_backward z");
+            require_rows(*z, "activation_backward z");
+            require_same(*z, *dz, "activation_backward z");
+        } else {
+            require_checkpoint(values, exponents, *dz, "activation_backward checkpoint");
+        }
+        int64_t partial_rows = 0;
+        if (partial != nullptr) {
+            check_tensor(partial, "activation_backward partial");
+            require_dtype(*partial, TPB_F32, "activation_backward partial");
+            partial_rows = partial->sizes[0];
+            TPB_CHECK(partial->ndim == 2 && is_contiguous(*partial) && partial_rows >= 1 && partial_rows <= 65535 &&
+                          partial->sizes[1] == (gated ? 2 : 1) * n,
+                      "activation_backward: partial sums are [1 .. 65535, parts * n], contiguous");
+        }
+        if (n == 0 || (m == 0 && partial == nullptr)) return;
+        const int dev = device_of(partial != nullptr ? partial->data : dz->data);
+        DeviceGuard guard(dev);
+        cudaStream_t s = resolve_stream(stream, dev);
+        TPB_DISPATCH_FFN(dz->dtype, "activation_backward", {
+            BackwardParams<scalar_t> p{};
+            p.dy = static_cast<const scalar_t*>(dy->data);
+            p.sdy_m = dy->strides[0];
+            if (z != nullptr) {
+                p.z = static_cast<const scalar_t*>(z->data);
+                p.sz_m = z->strides[0];
+                p.sz_p = gated ? z->strides[1] : 0;
+            } else {
+                p.values = static_cast<const int8_t*>(values->data);
+                p.exponents = static_cast<const uint8_t*>(exponents->data);
+                p.nb = (n + kCkptBlock - 1) / kCkptBlock;
+            }
+            p.dz = static_cast<scalar_t*>(dz->data);
+            p.sdz_m = dz->strides[0];
+            p.sdz_p = gated ? dz->strides[1] : 0;
+            if (partial != nullptr) p.partial = static_cast<float*>(partial->data);
+            p.m = m;
+            p.n = n;
+            p.act = act;
+            if (gated) dispatch_backward<scalar_t, true>(p, partial_rows, dev, s);
+            else dispatch_backward<scalar_t, false>(p, partial_rows, dev, s);
+        });
+    });
+}
+
+int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
+                              void* stream) {
+    return guarded([&] {
+        check_tensor(y, "checkpoint_unpack y");
+        require_float(*y, "checkpoint_unpack y");
+        TPB_CHECK(y->ndim == 2, "checkpoint_unpack: the result is [rows, n]");
+        require_rows(*y, "checkpoint_unpack y");
+        require_checkpoint(values, exponents, *y, "checkpoint_unpack");
+        const int64_t m = y->sizes[0], n = y->sizes[1];
+        if (m == 0 || n == 0) return;
+        const int dev = device_of(y->data);
+        DeviceGuard guard(dev);
+        cudaStream_t s = resolve_stream(stream, dev);
+        TPB_DISPATCH_FFN(y->dtype, "checkpoint_unpack", {
+            UnpackParams<scalar_t> p{};
+            p.y = static_cast<scalar_t*>(y->data);
+            p.sy_m = y->strides[0];
+            p.values = static_cast<const int8_t*>(values->data);
+            p.exponents = static_cast<const uint8_t*>(exponents->data);
+            p.n = n;
+            p.units = make_units(m, n);
+            if (n % 8 == 0 && rows16(p.y, p.sy_m, sizeof(scalar_t)) && reinterpret_cast<uintptr_t>(p.values) % 8 == 0) {
+                launch_pdl(checkpoint_unpack_kernel<scalar_t, 8>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
+            } else {
+                launch_pdl(checkpoint_unpack_kernel<scalar_t, 1>, unit_blocks(p.units, 32, 4), kThreads, 0, s, p);
+            }
+            check_launch("checkpoint_unpack");
+        });
+    });
+}
+
+}  // extern "C"

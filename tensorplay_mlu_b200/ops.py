@@ -1020,6 +1020,291 @@ def layer_norm(input, normalized_shape, weight=None, bias=None, eps: float = 1e-
     return native_layer_norm(input, normalized_shape, weight, bias, eps)[0]
 
 
+# ------------------------------------------------------------- feed-forward
+#
+# The gated feed-forward block, a linear layer with its activation and the
+# residual stream, and 8-bit checkpoints of what their backward passes need.
+# Not among the reference's registrations (there they are sequences of linear,
+# an activation, mul and add), so they stand outside KERNELS.
+
+_FFN_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _activation_code(activation: str, what: str) -> int:
+    try:
+        return N.ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise RuntimeError(f"{what}: activation must be one of {', '.join(N.ACTIVATIONS)}, got {activation!r}") from None
+
+
+def _ffn_check(what: str, x, *others) -> None:
+    """Device tensors on one device, in one supported dtype."""
+    if not _is_device(x):
+        _require_device(x)
+    if x.dtype not in _FFN_DTYPES:
+        raise RuntimeError(f"{what}: expected bfloat16, float16 or float32, got {x.dtype}")
+    for t in others:
+        if t is None:
+            continue
+        _require_device(t)
+        if t.dtype != x.dtype:
+            raise RuntimeError(f"{what}: expected operands of one dtype, got {x.dtype} and {t.dtype}")
+        if t.device != x.device:
+            raise RuntimeError(f"{what}: operands are on different devices")
+
+
+def _rows(t: torch.Tensor, rows: int, n: int) -> torch.Tensor:
+    """``t`` seen as [rows, n] with unit column stride (rows may be strided; copied when they cannot be)."""
+    if t.dim() == 2 and (t.stride(1) == 1 or n <= 1):
+        return t
+    return _dense(t).view(rows, n)
+
+
+def _product_rows(t: torch.Tensor) -> torch.Tensor:
+    """A 2-d operand of a tensor-core product: itself when its rows start on
+    16-byte boundaries (what a tensor-map load needs), otherwise a copy whose
+    rows do (one pass over it, instead of a product on the CUDA cores)."""
+    per = 16 // t.element_size()
+    if (t.data_ptr() % 16 == 0 and t.stride(0) % per == 0 and t.stride(0) > 0) or t.numel() == 0:
+        return t
+    pitch = (t.shape[1] + per - 1) // per * per
+    out = _empty((t.shape[0], pitch), t.dtype, t.device)[:, :t.shape[1]]
+    N.check(_lib().tp_b200_copy(describe(out), describe(t), _stream(t)), "copy")
+    return out
+
+
+def _layer_operands(what: str, input, weight, bias, parts: int):
+    """(x [rows, K], rows, out features per part, leading shape) of a linear layer, checked."""
+    _ffn_check(what, input, weight, bias)
+    if input.dim() == 0 or weight.dim() != 2:
+        raise RuntimeError(f"{what}: expected [..., K] input and 2-d weight, got {list(input.shape)} and "
+                           f"{list(weight.shape)}")
+    k, out = input.shape[-1], weight.shape[0]
+    if weight.shape[1] != k:
+        raise RuntimeError(f"{what}: input features {k} do not match the weight's {weight.shape[1]}")
+    if out % parts:
+        raise RuntimeError(f"{what}: the weight needs an even number of rows (gate rows, then up rows), got {out}")
+    if bias is not None and list(bias.shape) != [out]:
+        raise RuntimeError(f"{what}: expected a bias of {out} elements, got {list(bias.shape)}")
+    lead = input.shape[:-1]
+    rows = math.prod(lead)
+    return _rows(input, rows, k), rows, out // parts, lead
+
+
+def _checkpoint_empty(shape, device):
+    blocks = (shape[-1] + N.CHECKPOINT_BLOCK - 1) // N.CHECKPOINT_BLOCK
+    return (torch.empty(shape, dtype=torch.int8, device=device),
+            torch.empty((*shape[:-1], blocks), dtype=torch.uint8, device=device))
+
+
+def _checkpoint_check(what: str, values, exponents, shape, device) -> None:
+    _require_device(values, exponents)
+    if values.dtype != torch.int8 or exponents.dtype != torch.uint8:
+        raise RuntimeError(f"{what}: a checkpoint is int8 values and uint8 exponents, got {values.dtype} and "
+                           f"{exponents.dtype}")
+    blocks = (shape[-1] + N.CHECKPOINT_BLOCK - 1) // N.CHECKPOINT_BLOCK if len(shape) else 0
+    if list(values.shape) != list(shape) or list(exponents.shape) != [*shape[:-1], blocks]:
+        raise RuntimeError(f"{what}: a checkpoint of shape {list(shape)} has values of that shape and exponents "
+                           f"{[*shape[:-1], blocks]}, got {list(values.shape)} and {list(exponents.shape)}")
+    if values.device != device or exponents.device != device:
+        raise RuntimeError(f"{what}: operands are on different devices")
+
+
+def checkpoint_pack(x):
+    """An activation kept in 8 bits for the backward pass: ``(values, exponents)``.
+
+    Blocks of 32 consecutive elements of the last dimension share a power of
+    two: ``values`` (int8, x's shape) times ``2 ** (exponents - 127)``
+    (uint8, one per block), the least power for which the block fits, each
+    value rounded to nearest, ties to even.  The error is at most half that
+    power of two, 1/127 of the block's largest magnitude at worst.  A block
+    that holds an infinity or a NaN reads back as NaN."""
+    _ffn_check("checkpoint_pack", x)
+    if x.dim() == 0:
+        raise RuntimeError("checkpoint_pack: expected at least one dimension")
+    n = x.shape[-1]
+    values, exponents = _checkpoint_empty(tuple(x.shape), x.device)
+    if x.numel():
+        rows = x.numel() // n
+        N.check(_lib().tp_b200_activation_forward(
+            None, describe(values.view(rows, n)), describe(exponents.view(rows, -1)), describe(_rows(x, rows, n)), None,
+            0, _stream(x)), "checkpoint_pack")
+    return values, exponents
+
+
+def checkpoint_unpack(values, exponents, dtype: torch.dtype):
+    """The tensor an 8-bit checkpoint stands for, in ``dtype`` (exact in
+    bfloat16 and float32; float16 underflows below its subnormals)."""
+    _require_device(values)
+    if dtype not in _FFN_DTYPES:
+        raise RuntimeError(f"checkpoint_unpack: expected bfloat16, float16 or float32, got {dtype}")
+    if values.dim() == 0:
+        raise RuntimeError("checkpoint_unpack: expected at least one dimension")
+    _checkpoint_check("checkpoint_unpack", values, exponents, tuple(values.shape), values.device)
+    out = _empty(values.shape, dtype, values.device)
+    if out.numel():
+        n = values.shape[-1]
+        rows = out.numel() // n
+        N.check(_lib().tp_b200_checkpoint_unpack(
+            describe(out.view(rows, n)), describe(_dense(values).view(rows, n)),
+            describe(_dense(exponents).view(rows, -1)), _stream(values)), "checkpoint_unpack")
+    return out
+
+
+def checkpoint_activation_backward(grad_output, values, exponents, activation: str):
+    """``grad_output * act'(z)`` for an activation whose input z was kept as an 8-bit checkpoint."""
+    what = "checkpoint_activation_backward"
+    code = _activation_code(activation, what)
+    _ffn_check(what, grad_output)
+    _checkpoint_check(what, values, exponents, tuple(grad_output.shape), grad_output.device)
+    if grad_output.dim() == 0:
+        raise RuntimeError(f"{what}: expected at least one dimension")
+    out = _empty(grad_output.shape, grad_output.dtype, grad_output.device)
+    if out.numel():
+        n = out.shape[-1]
+        rows = out.numel() // n
+        N.check(_lib().tp_b200_activation_backward(
+            describe(out.view(rows, n)), None, describe(_rows(grad_output, rows, n)), None,
+            describe(_dense(values).view(rows, n)), describe(_dense(exponents).view(rows, -1)), code,
+            _stream(grad_output)), what)
+    return out
+
+
+def _layer_forward(what: str, input, weight, bias, residual, activation, parts: int, save: bool, checkpoint: bool):
+    code = _activation_code(activation, what)
+    x, rows, n, lead = _layer_operands(what, input, weight, bias, parts)
+    if residual is not None:
+        _ffn_check(what, input, residual)
+        if list(residual.shape) != [*lead, n]:
+            raise RuntimeError(f"{what}: expected a residual of the result's shape {[*lead, n]}, got "
+                               f"{list(residual.shape)}")
+        residual = _rows(residual, rows, n)
+    dev = x.device
+    y = _empty((*lead, n), x.dtype, dev)
+    wide = (rows, 2, n) if parts == 2 else (rows, n)
+    values = exponents = None
+    if checkpoint:
+        values, exponents = _checkpoint_empty(wide, dev)
+    z = None
+    if rows and n:
+        z = _empty(wide, x.dtype, dev)
+        _gemm(z.view(rows, parts * n), _product_rows(x), _product_rows(weight).t(), bias, 1.0,
+              1.0 if bias is not None else 0.0)
+        N.check(_lib().tp_b200_activation_forward(
+            describe(y.view(rows, n)), describe(values) if checkpoint else None,
+            describe(exponents) if checkpoint else None, describe(z),
+            describe(residual) if residual is not None else None, code, _stream(x)), what)
+    elif save and not checkpoint:
+        z = _empty(wide, x.dtype, dev)
+    if checkpoint:
+        saved = (values.view(*lead, *wide[1:]), exponents.view(*lead, *exponents.shape[1:]))
+    else:
+        saved = z.view(*lead, *wide[1:]) if save else None
+    return y, saved
+
+
+def _layer_backward(what: str, grad_output, input, weight, saved, activation, parts: int, output_mask):
+    code = _activation_code(activation, what)
+    x, rows, n, lead = _layer_operands(what, input, weight, None, parts)
+    _ffn_check(what, input, grad_output)
+    if list(grad_output.shape) != [*lead, n]:
+        raise RuntimeError(f"{what}: expected a gradient of shape {[*lead, n]}, got {list(grad_output.shape)}")
+    dy = _rows(grad_output, rows, n)
+    wide = (rows, 2, n) if parts == 2 else (rows, n)
+    shape = (*lead, *wide[1:])
+    z = values = exponents = None
+    if isinstance(saved, (tuple, list)):
+        if len(saved) != 2:
+            raise RuntimeError(f"{what}: a checkpoint is (values, exponents)")
+        _checkpoint_check(what, saved[0], saved[1], shape, x.device)
+        values, exponents = (_dense(t).view(*wide[:-1], t.shape[-1]) for t in saved)
+    else:
+        _ffn_check(what, input, saved)
+        if saved is None or list(saved.shape) != list(shape):
+            raise RuntimeError(f"{what}: expected saved pre-activations of shape {list(shape)}, got "
+                               f"{None if saved is None else list(saved.shape)}")
+        z = _dense(saved).view(wide)
+    mask = list(output_mask) + [True] * (3 - len(output_mask))
+    dev, out = x.device, parts * n
+    dx = _empty(input.shape, x.dtype, dev) if mask[0] else None
+    dw = _empty(weight.shape, x.dtype, dev) if mask[1] else None
+    db = None
+    if not (mask[0] or mask[1] or mask[2]):
+        return None, None, None
+    if out == 0 or rows == 0:
+        for t in (dx, dw):
+            if t is not None and t.numel():
+                fill_(t, 0)
+        if mask[2]:
+            db = zeros_like(_empty((out,), x.dtype, dev))
+        return dx, dw, db
+    # dz [rows, parts * n] with rows on 16-byte boundaries, as the two products read it.
+    per = 16 // x.element_size()
+    pitch = (out + per - 1) // per * per
+    dz = _empty((rows, pitch), x.dtype, dev)[:, :out]
+    groups = min(max(rows // 16, 1), 128)
+    partial = _empty((groups, out), torch.float32, dev) if mask[2] else None
+    dzv = dz.unflatten(1, (2, n)) if parts == 2 else dz
+    N.check(_lib().tp_b200_activation_backward(
+        describe(dzv), describe(partial) if partial is not None else None, describe(dy),
+        describe(z) if z is not None else None, describe(values) if values is not None else None,
+        describe(exponents) if exponents is not None else None, code, _stream(x)), what)
+    if dx is not None and dx.numel():
+        _gemm(dx.view(rows, weight.shape[1]), dz, _product_rows(weight))
+    if dw is not None and dw.numel():
+        _gemm(dw, dz.t(), _product_rows(x))
+    if mask[2]:
+        db = _reduce(N.SUM, partial, [0], False, x.dtype)
+    return dx, dw, db
+
+
+def native_gated_linear(input, weight, bias=None, activation: str = "silu", checkpoint: bool = False):
+    """The first half of a gated feed-forward block, with what its backward pass needs: ``(h, saved)``.
+
+    ``weight`` is [2 F, K]: the gate projection's rows, then the up
+    projection's (``bias`` [2 F] alike); ``h = act(input @ Wg.T + bg) *
+    (input @ Wu.T + bu)``, [..., F].  ``saved`` is both pre-activations,
+    [..., 2, F], or with ``checkpoint`` their 8-bit checkpoint (see
+    :func:`checkpoint_pack`).  ``activation`` is none, relu, gelu, gelu_tanh
+    or silu; bfloat16, float16 or float32."""
+    return _layer_forward("native_gated_linear", input, weight, bias, None, activation, 2, True, checkpoint)
+
+
+def gated_linear(input, weight, bias=None, activation: str = "silu"):
+    """:func:`native_gated_linear` without the saved pre-activations."""
+    return _layer_forward("gated_linear", input, weight, bias, None, activation, 2, False, False)[0]
+
+
+def native_gated_linear_backward(grad_output, input, weight, saved, activation: str = "silu",
+                                 output_mask=(True, True, True)):
+    """(dinput, dweight, dbias) of :func:`native_gated_linear`, each None where ``output_mask`` says so.
+    ``saved`` is what the forward pass returned."""
+    return _layer_backward("native_gated_linear_backward", grad_output, input, weight, saved, activation, 2,
+                           output_mask)
+
+
+def native_linear_act(input, weight, bias=None, residual=None, activation: str = "none", checkpoint: bool = False):
+    """A linear layer, its activation and the residual stream in one operator: ``(y, saved)``.
+
+    ``y = act(input @ weight.T + bias) + residual`` (residual of y's shape);
+    ``saved`` is the pre-activation in y's dtype, or with ``checkpoint`` its
+    8-bit checkpoint."""
+    return _layer_forward("native_linear_act", input, weight, bias, residual, activation, 1, True, checkpoint)
+
+
+def linear_act(input, weight, bias=None, residual=None, activation: str = "none"):
+    """:func:`native_linear_act` without the saved pre-activation."""
+    return _layer_forward("linear_act", input, weight, bias, residual, activation, 1, False, False)[0]
+
+
+def native_linear_act_backward(grad_output, input, weight, saved, activation: str = "none",
+                               output_mask=(True, True, True)):
+    """(dinput, dweight, dbias) of :func:`native_linear_act`, each None where
+    ``output_mask`` says so; the residual's gradient is ``grad_output``."""
+    return _layer_backward("native_linear_act_backward", grad_output, input, weight, saved, activation, 1,
+                           output_mask)
+
+
 # -------------------------------------------------------------------- index
 
 _SCATTER_MODES = {None: 0, "": 0, "add": 1, "sum": 1, "multiply": 2, "prod": 2, "amax": 3, "amin": 4,
