@@ -422,6 +422,19 @@ enum tpb_activation {
     TPB_ACT_SILU = 4
 };
 
+/* y [M, N] = act(x w^T + bias) + residual, and the gated block's first half,
+ * y = act(x wg^T + bg) * (x wu^T + bu) with w = [wg; wu] [2 N, K] and bias
+ * [2 N], each in one kernel: sums, bias, activation and residual in fp32, one
+ * rounding at the end.  bfloat16 or float16; K >= 1; x and w with unit column
+ * stride and rows on 16-byte boundaries, y and residual with unit column
+ * stride.  saved (may be NULL): the pre-activations [M, N] or [M, 2, N];
+ * values / exponents (may be NULL): their 8-bit checkpoint instead. */
+int tp_b200_linear_act(const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
+                       const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w, const tpb_tensor* bias,
+                       const tpb_tensor* residual, int act, void* stream);
+int tp_b200_gated_linear(const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
+                         const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w, const tpb_tensor* bias,
+                         int act, void* stream);
 /* y = act(z) [+ residual] for z [rows, n], y = act(z0) * z1 [+ residual] for
  * z [rows, 2, n]; y [rows, n] may be NULL.  values / exponents (may be NULL)
  * receive the checkpoint of z.  Rows may be strided; computed in fp32 and

@@ -143,6 +143,8 @@ _SIGNATURES = {
     "tp_b200_nll_loss_backward": ([_T, _T, _T, _T, _T, _I, _I64, _P], _I),
     "tp_b200_dropout": ([_T, _T, _T, _D, ctypes.c_uint64, ctypes.c_uint64, _P], _I),
     "tp_b200_masked_scale": ([_T, _T, _T, _D, _P], _I),
+    "tp_b200_linear_act": ([_T, _T, _T, _T, _T, _T, _T, _T, _I, _P], _I),
+    "tp_b200_gated_linear": ([_T, _T, _T, _T, _T, _T, _T, _I, _P], _I),
     "tp_b200_activation_forward": ([_T, _T, _T, _T, _T, _I, _P], _I),
     "tp_b200_activation_backward": ([_T, _T, _T, _T, _T, _T, _I, _P], _I),
     "tp_b200_checkpoint_unpack": ([_T, _T, _T, _P], _I),

@@ -34,4 +34,30 @@ void gemm_simt(const GemmProblem& p, int dev, cudaStream_t stream);
 // (dtype, TMA alignment); nothing has been launched then.
 bool gemm_tc(const GemmProblem& p, int dev, cudaStream_t stream);
 
+// A feed-forward product (tp_b200_linear_act, tp_b200_gated_linear).  x [M, K]
+// and w [parts * N, K] with unit stride along K; parts 2: gate rows, then up
+// rows.  16-bit floats.
+struct FfnProblem {
+    int dtype;
+    int64_t M, N, K;
+    int parts;
+    const void* x;
+    int64_t sx_m;
+    const void* w;
+    int64_t sw_n;
+    void* y;  // [M, N]
+    int64_t sy_m;
+    const void* bias;      // [parts * N] or null
+    const void* residual;  // [M, N] or null
+    int64_t sres_m;
+    void* saved;           // [M, parts, N] contiguous or null
+    int8_t* values;        // the same in 8 bits, or null
+    uint8_t* exponents;
+    int act;
+};
+
+// False when x or w does not fit the tensor maps (rows off 16-byte
+// boundaries) or K is 0; nothing has been launched then.
+bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream);
+
 }  // namespace tpb

@@ -1,0 +1,309 @@
+// The feed-forward products on tcgen05 tensor cores: a linear layer with its
+// bias, activation and residual, and the gated block's two projections with
+// the activation and their product (no single counterpart in the reference;
+// see include/tpb200.h).
+//
+// Both are the CTA-pair kernel of gemm_tc.cuh with another epilogue, so the
+// pre-activations stay in TMEM: written out, they would cost the gated block
+// 8 M F bytes of traffic (written, read back) beside the 2 M F of its result.
+//   * linear_act: a 256 x 256 tile of x W^T, as in a plain product.
+//   * gated_linear: the pair's tile is 256 rows by 128 gate and 128 up
+//     columns; the leader CTA stages the gate rows of W and its peer the up
+//     rows, so each CTA's accumulator holds both pre-activations of its 128
+//     rows (columns 0-127 and 128-255) and the epilogue multiplies them
+//     without an exchange.  The mainloop is the plain product's.
+// Sums, bias, activation, gate and residual are fp32; the result is rounded
+// once.  Pre-activations saved for the backward pass are rounded to T, or to
+// 8 bits (act.cuh): a TMEM lane is a row and a 32-column chunk is exactly one
+// checkpoint block, so its scale is found in one thread's registers.
+
+#include "act.cuh"
+#include "gemm_tc.cuh"
+
+namespace tpb {
+namespace {
+
+// Byte of element (row r, column c) in a warp's 32 x 32 staging tile of
+// 16-bit elements (64-byte-swizzled rows) or bytes (32-byte-swizzled rows).
+__device__ __forceinline__ int stage_offset16(int r, int c) {
+    return r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2;
+}
+__device__ __forceinline__ int stage_offset8(int r, int c) {
+    return r * 32 + (((c >> 4) ^ ((r >> 2) & 1)) << 4) + (c & 15);
+}
+
+// A staged 32 x 32 tile to rows that TMA cannot store (off 16-byte
+// boundaries): a row at a time, one element a lane.
+template <typename T>
+__device__ __forceinline__ void store_staged_rows(const uint8_t* stage, int lane, T* dst, int64_t pitch, int64_t cols,
+                                                  int64_t rows) {
+    for (int r = 0; r < 32; ++r) {
+        if (r < rows && lane < cols) {
+            const int at = sizeof(T) == 1 ? stage_offset8(r, lane) : stage_offset16(r, lane);
+            dst[r * pitch + lane] = *reinterpret_cast<const T*>(stage + at);
+        }
+    }
+}
+
+// ... and the residual's rows into one.
+template <typename T>
+__device__ __forceinline__ void load_staged_rows(uint8_t* stage, int lane, const T* src, int64_t pitch, int64_t cols,
+                                                 int64_t rows) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        const T v = r < rows && lane < cols ? src[r * pitch + lane] : T(0.0f);
+        *reinterpret_cast<T*>(stage + stage_offset16(r, lane)) = v;
+    }
+}
+
+// bias[n .. n + 32) added to a chunk (every lane reads the same addresses).
+template <typename T>
+__device__ __forceinline__ void add_bias_chunk(const T* bias, int64_t n, int64_t N, float (&z)[32]) {
+    if (n + 32 <= N && (reinterpret_cast<uintptr_t>(bias + n) & 15u) == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float f[8];
+            unpack_vec(reinterpret_cast<const Vec<T, 8>*>(bias + n)[q], f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[q * 8 + j] += f[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (n + j < N) z[j] += load_as<float>(bias[n + j]);
+        }
+    }
+}
+
+// One row's 32-element block as int8 into a staging tile; returns the
+// exponent.
+template <typename T>
+__device__ __forceinline__ uint8_t stage_checkpoint(uint8_t* stage, int lane, const float (&z)[32]) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) amax = max_nan(amax, fabsf(z[j]));
+    float qmax;
+    const int stored = ckpt_exponent<T>(amax, qmax);
+    const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        Vec<int8_t, 16> q;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) q.v[j] = ckpt_quantise(z[h * 16 + j], inverse, qmax);
+        *reinterpret_cast<Vec<int8_t, 16>*>(stage + stage_offset8(lane, h * 16)) = q;
+    }
+    return static_cast<uint8_t>(stored);
+}
+
+// Rows [row0, row0 + 32) (this warp's TMEM lanes) of one accumulator.  half:
+// which half of the tile's result columns this warp stores, in chunks of 32.
+template <typename T, int EPI>
+__device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUtensorMap* tmSaved, uint8_t* stage,
+                          uint32_t t_rows, int half, int64_t row0, int64_t n_tile0) {
+    constexpr int kParts = EPI == kEpiGated ? 2 : 1;
+    constexpr int kCols = pair_tile_columns<EPI>() / 2;
+    const FfnParams& f = p.ffn;
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = p.M - row0;
+    const T* bias = static_cast<const T*>(f.bias);
+    uint8_t* stage2 = stage + staging_bytes<T>();
+    for (int c0 = half * kCols; c0 < (half + 1) * kCols; c0 += 32) {
+        const int64_t n = n_tile0 + c0;
+        if (rows <= 0 || n >= p.N) break;
+        const int64_t cols = p.N - n;
+        uint32_t raw[kParts][32];
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) tmem_ld32(t_rows + c0 + q * 128, raw[q]);
+        // The residual's loads are in flight while the accumulator arrives.
+        Vec<T, 8> res[4];
+        bool res_vec = false;
+        if (f.residual != nullptr && lane < rows) {
+            const T* r = static_cast<const T*>(f.residual) + (row0 + lane) * f.sres_m + n;
+            res_vec = f.residual_vec && cols >= 32;
+            if (res_vec) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) res[q] = reinterpret_cast<const Vec<T, 8>*>(r)[q];
+            }
+        }
+        tmem_wait_ld();
+        float z[kParts][32];
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[q][j] = __uint_as_float(raw[q][j]);
+            if (bias != nullptr) add_bias_chunk<T>(bias + q * p.N, n, p.N, z[q]);
+            if (cols < 32) {  // columns past N hold other rows of W, or nothing
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    if (j >= cols) z[q][j] = 0.0f;
+                }
+            }
+        }
+        // The previous stores from the staging tiles have finished reading.
+        if (lane == 0) bulk_wait_group_read0();
+        __syncwarp();
+        if (f.saved != nullptr) {
+            // Two tiles: z into the second (gate into the first, which the
+            // result takes over once it has been read).
+            uint8_t* tile[2] = {kParts == 2 ? stage : stage2, stage2};
+#pragma unroll
+            for (int q = 0; q < kParts; ++q) {
+                Vec<T, 32> packed;
+                pack_vec(z[q], packed);
+                stage_chunk<T>(tile[q], lane, packed);
+            }
+            if (f.saved_tma) fence_proxy_async_smem();
+            __syncwarp();
+            if (f.saved_tma) {
+                if (lane == 0) {
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) tma_store_3d(tmSaved, smem_addr(tile[q]), int(n), q, int(row0));
+                    bulk_commit_group();
+                    if (kParts == 2) bulk_wait_group_read0();
+                }
+            } else {
+                T* dst = static_cast<T*>(f.saved) + row0 * f.ssaved_m + n;
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    store_staged_rows<T>(tile[q], lane, dst + q * f.ssaved_p, f.ssaved_m, cols, rows);
+                }
+            }
+            if (kParts == 2) __syncwarp();
+        } else if (f.values != nullptr) {
+#pragma unroll
+            for (int q = 0; q < kParts; ++q) {
+                const uint8_t stored = stage_checkpoint<T>(stage2 + q * 1024, lane, z[q]);
+                if (lane < rows) f.exponents[((row0 + lane) * kParts + q) * f.nb + (n >> 5)] = stored;
+            }
+            if (!f.saved_tma) {
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    store_staged_rows<int8_t>(stage2 + q * 1024, lane, f.values + (row0 * kParts + q) * p.N + n,
+                                              int64_t(kParts) * p.N, cols, rows);
+                }
+            }
+        }
+        act_values<true, 32>(f.act, z[0]);
+        if constexpr (kParts == 2) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[0][j] *= z[1][j];
+        }
+        if (f.residual != nullptr) {
+            if (f.residual_vec && cols >= 32) {
+                if (res_vec) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float r[8];
+                        unpack_vec(res[q], r);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) z[0][q * 8 + j] += r[j];
+                    }
+                }
+            } else {
+                load_staged_rows<T>(stage, lane, static_cast<const T*>(f.residual) + row0 * f.sres_m + n, f.sres_m, cols,
+                                    rows);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    z[0][j] += load_as<float>(*reinterpret_cast<const T*>(stage + stage_offset16(lane, j)));
+                }
+                __syncwarp();
+            }
+        }
+        Vec<T, 32> packed;
+        pack_vec(z[0], packed);
+        stage_chunk<T>(stage, lane, packed);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            if (p.tma_store) tma_store_2d(tmC, smem_addr(stage), int(n), int(row0));
+            if (f.values != nullptr && f.saved_tma) {
+#pragma unroll
+                for (int q = 0; q < kParts; ++q) {
+                    tma_store_3d(tmSaved, smem_addr(stage2 + q * 1024), int(n), q, int(row0));
+                }
+            }
+            bulk_commit_group();
+        }
+        if (!p.tma_store) {
+            store_staged_rows<T>(stage, lane, static_cast<T*>(p.c) + row0 * p.sc_m + n, p.sc_m, cols, rows);
+            __syncwarp();
+        }
+    }
+}
+
+// Map of [M, parts, N] for the saved tensors' TMA stores: boxes of 32 columns
+// of one part by 32 rows.
+CUtensorMap make_saved_map(void* base, CUtensorMapDataType type, int es, int64_t N, int64_t parts, int64_t M,
+                           int64_t part_stride, int64_t row_stride) {
+    CUtensorMap map;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(parts), static_cast<cuuint64_t>(M)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(part_stride * es), static_cast<cuuint64_t>(row_stride * es)};
+    cuuint32_t box[3] = {32, 1, 32};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = encode_fn()(&map, type, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   es == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    TPB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (saved) failed (%d)", static_cast<int>(r));
+    return map;
+}
+
+template <typename T>
+void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensorMapDataType type) {
+    constexpr int es = sizeof(T);
+    constexpr int kEPR = 128 / es;
+    const CUtensorMap ma = make_map(q.x, type, es, q.K, q.M, q.sx_m, 1, 0, kBoxRows);
+    const CUtensorMap mb = make_map(q.w, type, es, q.K, q.parts * q.N, q.sw_n, 1, 0, kBoxRows);
+    TcParams tp{};
+    tp.M = static_cast<int>(q.M);
+    tp.N = static_cast<int>(q.N);
+    tp.K = static_cast<int>(q.K);
+    tp.batch = 1;
+    tp.k_blocks = static_cast<int>((q.K + kEPR - 1) / kEPR);
+    tp.c = q.y;
+    tp.sc_m = q.sy_m;
+    tp.alpha = 1.0f;
+    tp.err = device_error_word(dev);
+    tp.tma_store = aligned16(q.y) && q.sy_m > 0 && (q.sy_m * es) % 16 == 0;
+    const CUtensorMap mc = tp.tma_store ? make_c_map(q.y, type, es, q.N, q.M, q.sy_m, 1, 0) : ma;
+    FfnParams& f = tp.ffn;
+    f.bias = q.bias;
+    f.residual = q.residual;
+    f.sres_m = q.sres_m;
+    f.residual_vec = aligned16(q.residual) && (q.sres_m * es) % 16 == 0;
+    f.act = q.act;
+    f.nb = (q.N + kCkptBlock - 1) / kCkptBlock;
+    CUtensorMap ms = ma;
+    if (q.saved != nullptr) {
+        f.saved = q.saved;
+        f.ssaved_m = q.parts * q.N;
+        f.ssaved_p = q.N;
+        f.saved_tma = aligned16(q.saved) && (q.N * es) % 16 == 0;
+        if (f.saved_tma) ms = make_saved_map(q.saved, type, es, q.N, q.parts, q.M, f.ssaved_p, f.ssaved_m);
+    } else if (q.values != nullptr) {
+        f.values = q.values;
+        f.exponents = q.exponents;
+        f.saved_tma = aligned16(q.values) && q.N % 16 == 0;
+        if (f.saved_tma) {
+            ms = make_saved_map(q.values, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.N, q.parts, q.M, q.N, q.parts * q.N);
+        }
+    }
+    if (q.parts == 2) launch_tc2<T, false, false, false, kEpiGated>(ma, mb, mc, tp, dev, stream, &ms);
+    else launch_tc2<T, false, false, false, kEpiAct>(ma, mb, mc, tp, dev, stream, &ms);
+}
+
+}  // namespace
+
+bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {
+    const int64_t limit = int64_t(1) << 30;
+    if (q.K == 0 || q.M >= limit || q.N >= limit || q.K >= limit) return false;
+    if (!tma_ok(q.x, 2, q.sx_m, 1, 0) || !tma_ok(q.w, 2, q.sw_n, 1, 0)) return false;
+    if (q.dtype == TPB_BF16) launch_ffn_pair<__nv_bfloat16>(q, dev, stream, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    else if (q.dtype == TPB_F16) launch_ffn_pair<__half>(q, dev, stream, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    else return false;
+    return true;
+}
+
+}  // namespace tpb

@@ -138,6 +138,21 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint
 
 // ------------------------------------------------------------ kernel --
 
+// The feed-forward epilogues' operands (kEpiAct, kEpiGated; gemm_ffn.cu).
+struct FfnParams {
+    const void* bias;      // [parts * N] or null
+    const void* residual;  // [M, N], row stride sres_m, or null
+    int64_t sres_m;
+    void* saved;           // pre-activations [M, parts, N] in T, or null
+    int64_t ssaved_m, ssaved_p;
+    int8_t* values;        // their 8-bit checkpoint (contiguous), or null
+    uint8_t* exponents;
+    int64_t nb;            // checkpoint blocks of a row
+    int act;
+    int residual_vec;      // residual rows on 16-byte boundaries
+    int saved_tma;         // saved / values are written by TMA stores
+};
+
 struct TcParams {
     int M, N, K, batch;
     int m_tiles, n_tiles, k_blocks, num_tiles;
@@ -164,6 +179,7 @@ struct TcParams {
     // evict_normal (A/B measurements).
     int l2_operands, l2_stream;
     int* err;
+    FfnParams ffn;
 };
 
 // Epilogue forms (template argument of the CTA-pair kernel).
@@ -179,6 +195,12 @@ struct TcParams {
 constexpr int kEpiPlain = 0;
 constexpr int kEpiGelu = 1;
 constexpr int kEpiGeluBackward = 2;
+//   kEpiAct           z = acc + bias; C = act(z) + residual; z kept in T, or
+//                     as an 8-bit checkpoint
+//   kEpiGated         the tile's 256 columns are 128 gate and 128 up columns:
+//                     C = act(zg) * zu over 128 columns; zg, zu kept alike
+constexpr int kEpiAct = 3;
+constexpr int kEpiGated = 4;
 
 // Element traits: 128 bytes of K per stage row in every case.
 template <typename T> struct TcElem;
@@ -506,6 +528,12 @@ __device__ __forceinline__ void store_accumulator_tma(const TcParams& p, const C
     }
 }
 
+// The feed-forward epilogues' store of one accumulator (defined in gemm_ffn.cu,
+// the only unit that instantiates kEpiAct / kEpiGated).
+template <typename T, int EPI>
+__device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUtensorMap* tmSaved, uint8_t* stage,
+                          uint32_t t_rows, int half, int64_t row0, int64_t n_tile0);
+
 // ------------------------------------------------- 2-SM (CTA pair) kernel --
 //
 // A cluster of two CTAs on two SMs computes a 256 x 256 tile with
@@ -593,7 +621,13 @@ constexpr int kPairBN = 256;  // columns per CTA pair (each CTA stages 128 of B)
 // Staging tiles per epilogue warp: two when the epilogue writes two results.
 template <int EPI>
 __host__ __device__ constexpr int staging_tiles() {
-    return EPI == kEpiGelu ? 2 : 1;
+    return EPI == kEpiGelu || EPI == kEpiAct || EPI == kEpiGated ? 2 : 1;
+}
+
+// Result columns of one CTA-pair tile.
+template <int EPI>
+__host__ __device__ constexpr int pair_tile_columns() {
+    return EPI == kEpiGated ? 128 : kPairBN;
 }
 
 template <typename T, int EPI = kEpiPlain>
@@ -797,7 +831,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTc2Threads, 1)
                 int b, mt, nt;
                 tile_coords_pair(p, tile, b, mt, nt, group_m);
                 const int m0 = mt * kPairBM + int(rank) * 128;
-                const int n0 = nt * kPairBN + int(rank) * 128;
+                // kEpiGated: the leader stages the tile's 128 gate rows of the
+                // weight, the peer its 128 up rows, N further down.
+                const int n0 = EPI == kEpiGated ? nt * 128 + int(rank) * p.N : nt * kPairBN + int(rank) * 128;
                 const int kb_request = leader && p.sched != nullptr ? max(0, p.k_blocks - kClaimLead) : -1;
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
                     if (kb == kb_request) mbar_arrive(smem_addr(sched_req));  // claim the next tile now
@@ -944,7 +980,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTc2Threads, 1)
             tile_coords_pair(p, tile, b, mt, nt, group_m);
             const int64_t gm = int64_t(mt) * kPairBM + row_in_tile;
             const uint32_t t_rows = tmem_base + (uint32_t(quad * 32) << 16) + acc * kPairBN;
-            if (p.tma_store) {
+            if constexpr (EPI == kEpiAct || EPI == kEpiGated) {
+                store_ffn<T, EPI>(p, &tmC, &tmAux, staging + (warp - 2) * staging_tiles<EPI>() * staging_bytes<T>(),
+                                  t_rows, half, gm - lane, int64_t(nt) * pair_tile_columns<EPI>());
+            } else if (p.tma_store) {
                 uint8_t* stage = staging + (warp - 2) * staging_tiles<EPI>() * staging_bytes<T>();
                 store_accumulator_tma<T, kPairBN / 2, BATCHED, EPI>(p, &tmC, stage, t_rows, half * (kPairBN / 2), b,
                                                                     gm, gm - lane, int64_t(nt) * kPairBN, gm < p.M,
@@ -1043,7 +1082,7 @@ void launch_tc2(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap&
         configured[dev] = true;
     }
     tp.m_tiles = (tp.M + kPairBM - 1) / kPairBM;
-    tp.n_tiles = (tp.N + kPairBN - 1) / kPairBN;
+    tp.n_tiles = (tp.N + pair_tile_columns<EPI>() - 1) / pair_tile_columns<EPI>();
     tp.num_tiles = tp.batch * tp.m_tiles * tp.n_tiles;
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : std::is_same<T, float>::value ? 2u : 0u;
     tp.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(tp.a_mn) << 15) |

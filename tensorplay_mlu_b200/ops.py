@@ -1126,9 +1126,10 @@ def checkpoint_pack(x):
     values, exponents = _checkpoint_empty(tuple(x.shape), x.device)
     if x.numel():
         rows = x.numel() // n
+        x2 = _rows(x, rows, n)
         N.check(_lib().tp_b200_activation_forward(
-            None, describe(values.view(rows, n)), describe(exponents.view(rows, -1)), describe(_rows(x, rows, n)), None,
-            0, _stream(x)), "checkpoint_pack")
+            None, describe(values.view(rows, n)), describe(exponents.view(rows, -1)), describe(x2), None, 0, _stream(x)),
+            "checkpoint_pack")
     return values, exponents
 
 
@@ -1145,9 +1146,9 @@ def checkpoint_unpack(values, exponents, dtype: torch.dtype):
     if out.numel():
         n = values.shape[-1]
         rows = out.numel() // n
-        N.check(_lib().tp_b200_checkpoint_unpack(
-            describe(out.view(rows, n)), describe(_dense(values).view(rows, n)),
-            describe(_dense(exponents).view(rows, -1)), _stream(values)), "checkpoint_unpack")
+        values, exponents = _dense(values).view(rows, n), _dense(exponents).view(rows, -1)
+        N.check(_lib().tp_b200_checkpoint_unpack(describe(out.view(rows, n)), describe(values), describe(exponents),
+                                                 _stream(values)), "checkpoint_unpack")
     return out
 
 
@@ -1163,10 +1164,10 @@ def checkpoint_activation_backward(grad_output, values, exponents, activation: s
     if out.numel():
         n = out.shape[-1]
         rows = out.numel() // n
-        N.check(_lib().tp_b200_activation_backward(
-            describe(out.view(rows, n)), None, describe(_rows(grad_output, rows, n)), None,
-            describe(_dense(values).view(rows, n)), describe(_dense(exponents).view(rows, -1)), code,
-            _stream(grad_output)), what)
+        dy = _rows(grad_output, rows, n)
+        values, exponents = _dense(values).view(rows, n), _dense(exponents).view(rows, -1)
+        N.check(_lib().tp_b200_activation_backward(describe(out.view(rows, n)), None, describe(dy), None, describe(values),
+                                                   describe(exponents), code, _stream(dy)), what)
     return out
 
 
@@ -1185,17 +1186,31 @@ def _layer_forward(what: str, input, weight, bias, residual, activation, parts: 
     values = exponents = None
     if checkpoint:
         values, exponents = _checkpoint_empty(wide, dev)
-    z = None
-    if rows and n:
-        z = _empty(wide, x.dtype, dev)
+    z = _empty(wide, x.dtype, dev) if save and not checkpoint else None
+    if rows and n and x.dtype != torch.float32 and x.shape[1]:
+        # One kernel; the pre-activations stay on chip unless they are saved.
+        # (Copies made here are named: a descriptor does not keep its tensor alive.)
+        xp, wp = _product_rows(x), _product_rows(_rows(weight, parts * n, x.shape[1]))
+        bp = _dense(bias) if bias is not None else None
+        args = [describe(y.view(rows, n)), describe(z) if z is not None else None,
+                describe(values) if checkpoint else None, describe(exponents) if checkpoint else None,
+                describe(xp), describe(wp), describe(bp) if bp is not None else None]
+        if parts == 2:
+            status = _lib().tp_b200_gated_linear(*args, code, _stream(x))
+        else:
+            status = _lib().tp_b200_linear_act(*args, describe(residual) if residual is not None else None, code,
+                                               _stream(x))
+        N.check(status, what)
+    elif rows and n:
+        # float32 (whose products are several launches), or no input features.
+        if z is None:
+            z = _empty(wide, x.dtype, dev)
         _gemm(z.view(rows, parts * n), _product_rows(x), _product_rows(weight).t(), bias, 1.0,
               1.0 if bias is not None else 0.0)
         N.check(_lib().tp_b200_activation_forward(
             describe(y.view(rows, n)), describe(values) if checkpoint else None,
             describe(exponents) if checkpoint else None, describe(z),
             describe(residual) if residual is not None else None, code, _stream(x)), what)
-    elif save and not checkpoint:
-        z = _empty(wide, x.dtype, dev)
     if checkpoint:
         saved = (values.view(*lead, *wide[1:]), exponents.view(*lead, *exponents.shape[1:]))
     else:
