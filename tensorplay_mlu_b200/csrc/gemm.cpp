@@ -184,7 +184,16 @@ int feed_forward(const char* what, int parts, const tpb_tensor* y, const tpb_ten
         q.parts = parts;
         require_matrix(y, q.dtype, q.M, q.N, what);
         require_matrix(x, q.dtype, q.M, q.K, what);
-        require_matrix(w, q.dtype, parts * q.N, q.K, what);
+        check_tensor(w, what);
+        TPB_CHECK(w->dtype == q.dtype && w->ndim == 2 && w->sizes[0] == parts * q.N && w->sizes[1] == q.K,
+                  "%s: expected a weight [%lld, %lld] of the result's dtype", what, (long long)(parts * q.N),
+                  (long long)q.K);
+        // A weight with unit stride along its rows instead is read in place
+        // where no epilogue is asked for (the input gradient dz W).
+        const bool unit_k = w->strides[1] == 1 || (q.K == 1 && w->strides[0] != 1);
+        q.w_transposed = !unit_k && w->strides[0] == 1 && parts == 1 && bias == nullptr && residual == nullptr &&
+                         saved == nullptr && values == nullptr && act == TPB_ACT_NONE;
+        TPB_CHECK(unit_k || q.w_transposed, "%s: the weight needs unit column stride", what);
         TPB_CHECK(q.K > 0, "%s: needs at least one input feature", what);
         if (bias != nullptr) {
             check_tensor(bias, what);
@@ -214,7 +223,7 @@ int feed_forward(const char* what, int parts, const tpb_tensor* y, const tpb_ten
         q.x = x->data;
         q.sx_m = x->strides[0];
         q.w = w->data;
-        q.sw_n = w->strides[0];
+        q.sw_n = w->strides[q.w_transposed ? 1 : 0];
         q.y = y->data;
         q.sy_m = y->strides[0];
         q.act = act;

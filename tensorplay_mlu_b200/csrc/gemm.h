@@ -45,6 +45,7 @@ struct FfnProblem {
     int64_t sx_m;
     const void* w;
     int64_t sw_n;
+    int w_transposed;  // w is [K, N] with unit stride along N (parts 1)
     void* y;  // [M, N]
     int64_t sy_m;
     const void* bias;      // [parts * N] or null
@@ -59,5 +60,7 @@ struct FfnProblem {
 // False when x or w does not fit the tensor maps (rows off 16-byte
 // boundaries) or K is 0; nothing has been launched then.
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream);
+// The same for few rows; x and w fit the tensor maps.
+void gemm_few(const FfnProblem& q, int dev, cudaStream_t stream);
 
 }  // namespace tpb

@@ -1,0 +1,432 @@
+// Feed-forward products for few rows (one token to a few hundred): the same
+// results as gemm_ffn.cu where its 256 x 256 tiles would leave most SMs idle
+// or compute mostly padding.
+//
+// With M rows the product reads the weight once (2 N K bytes in 16 bits) and
+// does 2 M N K operations, so up to M of about 250 its bound is HBM: every SM
+// has to stream weights all the time.  Hence
+//   * the weight is the MMA's 128-row operand and the rows of x its N
+//     dimension (kNT = 16 .. 128), so no tensor work goes into padding rows
+//     beyond the next 16;
+//   * a gated tile is 64 gate rows and 64 up rows of the weight, so both
+//     operators stage the same 128 rows and two CTAs fit an SM: one's set-up
+//     and final sum overlap the other's stream;
+//   * K is split over a cluster of C CTAs, because N / 128 tiles alone do not
+//     fill 148 SMs; each CTA streams its share of K through a TMA ring into
+//     TMEM accumulators;
+//   * the partial accumulators go to shared memory and each CTA of the cluster
+//     sums its share of the outputs over distributed shared memory, in rank
+//     order (the same bits on every run, no workspace, no atomics), then
+//     applies bias, activation, gate and residual in fp32.
+// The weight is read K-major (x W^T) or, for the input gradient dz W, in
+// place as an MN-major operand.
+//
+// Every wait is bounded as in gemm_tc.cu; all threads reach the cluster
+// barriers.  No TMA multicast is used.
+
+#include "act.cuh"
+#include "gemm_tc.cuh"
+
+namespace tpb {
+namespace {
+
+constexpr int kFewThreads = 192;  // warp 0 TMA producer, 1 MMA issuer, 2-5 accumulator readers
+constexpr int kFewWarps = kFewThreads / 32;
+
+struct FewParams {
+    int M, N, K;       // rows of x; result columns of one part; contraction
+    int k_blocks;
+    int row_tiles;     // ceil(M / kNT)
+    uint32_t idesc;
+    void* y;
+    int64_t sy_m;
+    FfnParams ffn;
+    int* err;
+};
+
+template <int NT>
+struct FewShape {
+    static constexpr uint32_t kWBytes = 128 * 128;
+    static constexpr uint32_t kXBytes = NT * 128;
+    static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
+    static constexpr int kCtas = 2;  // per SM, 110 KB of stages each
+    static constexpr int kStages = int(110 * 1024 / kStageBytes);
+    static constexpr uint32_t kPartialBytes = NT * 128 * 4;  // reuses the stages
+    static_assert(kPartialBytes <= kStages * kStageBytes, "partial sums fit the stages");
+    static constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024 + 256;
+    static constexpr int kTmemCols = NT < 32 ? 32 : NT;  // a power of two
+};
+
+// 32 lanes x 16 consecutive 32-bit columns of TMEM into 16 registers.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+template <int V>
+__device__ __forceinline__ void ld_cluster(uint32_t cluster_addr, float (&v)[V]) {
+    static_assert(V == 2 || V == 4, "8 or 16 bytes");
+    if constexpr (V == 4) {
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                     : "r"(cluster_addr)
+                     : "memory");
+    } else {
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(cluster_addr) : "memory");
+    }
+}
+
+// V consecutive elements of a row, vectorised where all of them exist on a
+// boundary of their size.
+template <typename T, int V>
+__device__ __forceinline__ void load_few(const T* src, int64_t left, float (&v)[V]) {
+    if (left >= V && reinterpret_cast<uintptr_t>(src) % (V * sizeof(T)) == 0) {
+        unpack_vec(*reinterpret_cast<const Vec<T, V>*>(src), v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = j < left ? load_as<float>(src[j]) : 0.0f;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_few(T* dst, int64_t left, const float (&v)[V]) {
+    if (left >= V && reinterpret_cast<uintptr_t>(dst) % (V * sizeof(T)) == 0) {
+        Vec<T, V> o;
+        pack_vec(v, o);
+        *reinterpret_cast<Vec<T, V>*>(dst) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (j < left) dst[j] = store_as<T>(v[j]);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+
+// V results of row m from column n on (a warp holds 32 V consecutive ones):
+// z[part] are their summed pre-activations.
+template <typename T, int PARTS, int V>
+__device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_t n, float (&z)[PARTS][V]) {
+    const FfnParams& f = p.ffn;
+    const int64_t left = p.N - n;  // may be negative
+    const T* bias = static_cast<const T*>(f.bias);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+        if (bias != nullptr && left > 0) {
+            float b[V];
+            load_few<T, V>(bias + int64_t(q) * p.N + n, left, b);
+#pragma unroll
+            for (int j = 0; j < V; ++j) z[q][j] += b[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {  // rows of the weight past this part
+            if (j >= left) z[q][j] = 0.0f;
+        }
+        if (f.saved != nullptr && left > 0) {
+            store_few<T, V>(static_cast<T*>(f.saved) + m * f.ssaved_m + q * f.ssaved_p + n, left, z[q]);
+        }
+        if (f.values != nullptr) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) amax = max_nan(amax, fabsf(z[q][j]));
+#pragma unroll
+            for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            float qmax;
+            const int stored = ckpt_exponent<T>(amax, qmax);
+            const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+            const int64_t row = m * PARTS + q;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (j < left) f.values[row * p.N + n + j] = ckpt_quantise(z[q][j], inverse, qmax);
+            }
+            if (n % kCkptBlock == 0 && left > 0) f.exponents[row * f.nb + n / kCkptBlock] = static_cast<uint8_t>(stored);
+        }
+    }
+    if (left <= 0) return;
+    act_values<true, V>(f.act, z[0]);
+    if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[0][j] *= z[1][j];
+    }
+    if (f.residual != nullptr) {
+        float r[V];
+        load_few<T, V>(static_cast<const T*>(f.residual) + m * f.sres_m + n, left, r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[0][j] += r[j];
+    }
+    store_few<T, V>(static_cast<T*>(p.y) + m * p.sy_m + n, left, z[0]);
+}
+
+template <typename T, int PARTS, int NT, bool W_MN>
+__global__ void __launch_bounds__(kFewThreads)
+    gemm_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const FewParams p) {
+    using S = FewShape<NT>;
+    constexpr int kStages = S::kStages;
+    constexpr int kColumns = 128 / PARTS;  // result columns of a tile
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * S::kStageBytes);
+    uint64_t* empty = full + kStages;
+    uint64_t* done = empty + kStages;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    pdl_trigger();
+    const int ranks = int(cluster_size());
+    const int rank = int(cluster_ctarank());
+    const int tile = blockIdx.x / ranks;
+    // Row tiles of one weight tile are neighbours, so its later readers hit L2.
+    const int wt = tile / p.row_tiles, mt = tile - wt * p.row_tiles;
+    const int n0 = wt * kColumns, m0 = mt * NT;
+    const int kb0 = int(int64_t(p.k_blocks) * rank / ranks), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / ranks);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_addr(&full[s]), 1);
+            mbar_init(smem_addr(&empty[s]), 1);
+        }
+        mbar_init(smem_addr(done), 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmW)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_addr(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(smem_addr(&empty[stage]), phase ^ 1, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t fb = smem_addr(&full[stage]);
+                const uint32_t at = smem_addr(smem + stage * S::kStageBytes);
+                mbar_expect_tx(fb, S::kStageBytes);
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    load_operand<2, W_MN, false, false>(at + q * (S::kWBytes / PARTS), &tmW, fb, n0 + q * p.N, kb * 64,
+                                                        0, kColumns);
+                }
+                tma_load_2d(at + S::kWBytes, &tmX, fb, kb * 64, m0);
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) {
+                atomicExch(p.err, kErrProducer);
+                // Loads already issued land before the CTA leaves.
+                for (int s = 0; s < kStages; ++s) {
+                    mbar_wait_bounded(smem_addr(&full[s]), (s < stage) ? phase : phase ^ 1);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t a_lbo = W_MN ? 8192 : 16;
+            constexpr uint32_t a_kstep = W_MN ? 16 * 128 : 32;
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(smem_addr(&full[stage]), phase, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t at = smem_addr(smem + stage * S::kStageBytes);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint64_t ad = sw128_desc(at + kk * a_kstep, a_lbo, 1024);
+                    const uint64_t bd = sw128_desc(at + S::kWBytes + kk * 32, 16, 1024);
+                    umma<false>(tmem, ad, bd, p.idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+                }
+                umma_commit(smem_addr(&empty[stage]));
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (!ok) atomicExch(p.err, kErrMma);
+            // The accumulators are complete (or, after a failure, every MMA
+            // issued is, so that TMEM can be released).
+            umma_commit(smem_addr(done));
+            if (!mbar_wait_bounded(smem_addr(done), 0)) atomicExch(p.err, kErrMma);
+        }
+    } else {
+        const int quad = warp & 3;  // the TMEM lanes this warp may read
+        if (!mbar_wait_bounded(smem_addr(done), 0)) {
+            if (lane == 0) atomicExch(p.err, kErrEpilogue);
+        } else {
+            tc_fence_after();
+            float* partial = reinterpret_cast<float*>(smem);
+#pragma unroll
+            for (int c = 0; c < NT; c += 16) {
+                if (c >= p.M - m0) break;  // rows of x past M
+                uint32_t r[16];
+                tmem_ld16(tmem + (uint32_t(quad * 32) << 16) + c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) partial[(c + j) * 128 + quad * 32 + lane] = __uint_as_float(r[j]);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // every CTA's partial sums are in its shared memory
+    tc_fence_after();
+    // partial[row of x][row of the weight tile]; a warp takes a row of x, a
+    // lane V columns of it, four ranks' loads in flight at a time.
+    constexpr int kV = kColumns / 32;
+    const int rows = min(NT, p.M - m0);
+    for (int m = rank + ranks * warp; m < rows; m += ranks * kFewWarps) {
+        float z[PARTS][kV];
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            const uint32_t at = smem_addr(smem) + uint32_t(m * 128 + q * kColumns + lane * kV) * 4;
+#pragma unroll
+            for (int j = 0; j < kV; ++j) z[q][j] = 0.0f;
+            for (int c0 = 0; c0 < ranks; c0 += 4) {
+                float v[4][kV];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c0 + c < ranks) ld_cluster<kV>(map_to_cta(at, uint32_t(c0 + c)), v[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c0 + c < ranks) {
+#pragma unroll
+                        for (int j = 0; j < kV; ++j) z[q][j] += v[c][j];
+                    }
+                }
+            }
+        }
+        finish_few<T, PARTS, kV>(p, m0 + m, int64_t(n0) + lane * kV, z);
+    }
+    cluster_sync();  // no CTA leaves while another reads its shared memory
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmemCols);
+    }
+}
+
+template <typename T, int PARTS, int NT, bool W_MN>
+void launch_few(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType type, FewParams& p, int dev,
+                cudaStream_t stream) {
+    using S = FewShape<NT>;
+    auto kern = gemm_few_kernel<T, PARTS, NT, W_MN>;
+    static bool configured[64] = {};
+    if (!configured[dev]) {
+        TPB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+        configured[dev] = true;
+    }
+    const CUtensorMap mx = make_map(q.x, type, 2, q.K, q.M, q.sx_m, 1, 0, NT);
+    const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(W_MN) << 15) | (uint32_t(NT >> 3) << 17) |
+              (uint32_t(128 >> 4) << 24);
+    p.row_tiles = (p.M + NT - 1) / NT;
+    const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
+    // K's split: the cluster size with the fewest k-blocks in a row, a CTA's
+    // set-up and its share of the sum counted as eight of them.
+    const int64_t slots = int64_t(gemm_sm_budget(dev)) * S::kCtas;
+    int split = 1;
+    int64_t best = INT64_MAX;
+    for (int c = 1; c <= 8 && c <= p.k_blocks; ++c) {
+        const int64_t waves = (tiles * c + slots - 1) / slots;
+        const int64_t cost = waves * ((p.k_blocks + c - 1) / c + 8);
+        if (cost < best) {
+            best = cost;
+            split = c;
+        }
+    }
+    static const int forced = std::getenv("TPB200_FFN_SPLIT") ? std::atoi(std::getenv("TPB200_FFN_SPLIT")) : 0;
+    if (forced > 0) split = std::min(forced, p.k_blocks);
+    TPB_CHECK(tiles * split < (int64_t(1) << 31), "feed-forward product: too many tiles");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = static_cast<unsigned>(tiles * split);
+    cfg.blockDim = kFewThreads;
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    TPB_CUDA(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
+    check_launch("gemm_few");
+}
+
+template <typename T, int PARTS, bool W_MN>
+void launch_rows(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType type, FewParams& p, int dev,
+                 cudaStream_t stream) {
+    if (q.M <= 16) launch_few<T, PARTS, 16, W_MN>(q, mw, type, p, dev, stream);
+    else if (q.M <= 32) launch_few<T, PARTS, 32, W_MN>(q, mw, type, p, dev, stream);
+    else if (q.M <= 64) launch_few<T, PARTS, 64, W_MN>(q, mw, type, p, dev, stream);
+    else launch_few<T, PARTS, 128, W_MN>(q, mw, type, p, dev, stream);
+}
+
+template <typename T>
+void launch_typed(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream) {
+    FewParams p{};
+    p.M = static_cast<int>(q.M);
+    p.N = static_cast<int>(q.N);
+    p.K = static_cast<int>(q.K);
+    p.k_blocks = static_cast<int>((q.K + 63) / 64);
+    p.y = q.y;
+    p.sy_m = q.sy_m;
+    p.err = device_error_word(dev);
+    FfnParams& f = p.ffn;
+    f.bias = q.bias;
+    f.residual = q.residual;
+    f.sres_m = q.sres_m;
+    f.saved = q.saved;
+    f.ssaved_m = q.parts * q.N;
+    f.ssaved_p = q.N;
+    f.values = q.values;
+    f.exponents = q.exponents;
+    f.nb = (q.N + kCkptBlock - 1) / kCkptBlock;
+    f.act = q.act;
+    if (q.w_transposed) {
+        const CUtensorMap mw = make_map(q.w, type, 2, q.N, q.K, q.sw_n, 1, 0, 64);
+        launch_rows<T, 1, true>(q, mw, type, p, dev, stream);
+    } else {
+        const CUtensorMap mw = make_map(q.w, type, 2, q.K, q.parts * q.N, q.sw_n, 1, 0, kBoxRows);
+        if (q.parts == 2) launch_rows<T, 2, false>(q, mw, type, p, dev, stream);
+        else launch_rows<T, 1, false>(q, mw, type, p, dev, stream);
+    }
+}
+
+}  // namespace
+
+void gemm_few(const FfnProblem& q, int dev, cudaStream_t stream) {
+    if (q.dtype == TPB_BF16) launch_typed<__nv_bfloat16>(q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dev, stream);
+    else launch_typed<__half>(q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dev, stream);
+}
+
+}  // namespace tpb

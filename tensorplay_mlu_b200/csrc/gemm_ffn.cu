@@ -296,13 +296,45 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
 
 }  // namespace
 
+// Whether the few-row kernel takes a product.
+bool few_rows(const FfnProblem& q, int) {
+    static const int limit = std::getenv("TPB200_FFN_FEW") ? std::atoi(std::getenv("TPB200_FFN_FEW")) : 128;
+    return q.M <= limit;
+}
+
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {
     const int64_t limit = int64_t(1) << 30;
     if (q.K == 0 || q.M >= limit || q.N >= limit || q.K >= limit) return false;
     if (!tma_ok(q.x, 2, q.sx_m, 1, 0) || !tma_ok(q.w, 2, q.sw_n, 1, 0)) return false;
-    if (q.dtype == TPB_BF16) launch_ffn_pair<__nv_bfloat16>(q, dev, stream, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
-    else if (q.dtype == TPB_F16) launch_ffn_pair<__half>(q, dev, stream, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
-    else return false;
+    TPB_CHECK(q.dtype == TPB_BF16 || q.dtype == TPB_F16, "feed-forward product: 16-bit floats only");
+    if (few_rows(q, dev)) {
+        gemm_few(q, dev, stream);
+    } else if (q.w_transposed) {
+        // Without an epilogue this is the plain product.
+        TPB_CHECK(q.bias == nullptr && q.residual == nullptr && q.saved == nullptr && q.values == nullptr &&
+                      q.act == TPB_ACT_NONE,
+                  "feed-forward product: a weight read transposed takes no epilogue at %lld rows", (long long)q.M);
+        GemmProblem p{};
+        p.dtype = q.dtype;
+        p.M = q.M;
+        p.N = q.N;
+        p.K = q.K;
+        p.batch = 1;
+        p.a = q.x;
+        p.sa_m = q.sx_m;
+        p.sa_k = 1;
+        p.b = q.w;
+        p.sb_k = q.sw_n;
+        p.sb_n = 1;
+        p.c = q.y;
+        p.sc_m = q.sy_m;
+        p.alpha = 1.0;
+        return gemm_tc(p, dev, stream);
+    } else if (q.dtype == TPB_BF16) {
+        launch_ffn_pair<__nv_bfloat16>(q, dev, stream, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    } else {
+        launch_ffn_pair<__half>(q, dev, stream, CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+    }
     return true;
 }
 

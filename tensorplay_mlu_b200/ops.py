@@ -1265,7 +1265,12 @@ def _layer_backward(what: str, grad_output, input, weight, saved, activation, pa
         describe(z) if z is not None else None, describe(values) if values is not None else None,
         describe(exponents) if exponents is not None else None, code, _stream(x)), what)
     if dx is not None and dx.numel():
-        _gemm(dx.view(rows, weight.shape[1]), dz, _product_rows(weight))
+        wp = _product_rows(_rows(weight, out, weight.shape[1]))
+        if x.dtype != torch.float32:
+            N.check(_lib().tp_b200_linear_act(describe(dx.view(rows, weight.shape[1])), None, None, None, describe(dz),
+                                              describe(wp.t()), None, None, 0, _stream(x)), what)
+        else:
+            _gemm(dx.view(rows, weight.shape[1]), dz, wp)
     if dw is not None and dw.numel():
         _gemm(dw, dz.t(), _product_rows(x))
     if mask[2]:
