@@ -422,19 +422,64 @@ enum tpb_activation {
     TPB_ACT_SILU = 4
 };
 
-/* y [M, N] = act(x w^T + bias) + residual, and the gated block's first half,
- * y = act(x wg^T + bg) * (x wu^T + bu) with w = [wg; wu] [2 N, K] and bias
- * [2 N], each in one kernel: sums, bias, activation and residual in fp32, one
- * rounding at the end.  bfloat16 or float16; K >= 1; x and w with unit column
- * stride and rows on 16-byte boundaries, y and residual with unit column
- * stride.  saved (may be NULL): the pre-activations [M, N] or [M, 2, N];
- * values / exponents (may be NULL): their 8-bit checkpoint instead. */
-int tp_b200_linear_act(const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
-                       const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w, const tpb_tensor* bias,
-                       const tpb_tensor* residual, int act, void* stream);
-int tp_b200_gated_linear(const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
-                         const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w, const tpb_tensor* bias,
-                         int act, void* stream);
+/* A linear layer with its activation: parts 1: y [m, n] = act(x w^T + bias) +
+ * residual, w [n, k]; parts 2, the gated block's first half: y = act(x wg^T +
+ * bg) * (x wu^T + bu), w = [wg; wu] [2 n, k], bias [2 n], no residual.  Each
+ * is one kernel for bfloat16 and float16: sums, bias, activation, gate and
+ * residual in fp32, one rounding at the end.  Matrices have unit column
+ * stride and the row strides given (elements); for bfloat16 and float16 the
+ * rows of x and w start on 16-byte boundaries.
+ *   saved       may be NULL: receives the pre-activations [m, n] / [m, 2, n].
+ *               float32, and k = 0, need it (their product is written there).
+ *   values, exponents   may be NULL: receive their 8-bit checkpoint.
+ *   bias, residual      may be NULL.
+ *   flags       as tp_b200_gemm (float32 products). */
+typedef struct tpb_layer {
+    int32_t dtype, act, parts, flags;
+    int64_t m, n, k;
+    const void* x;
+    int64_t x_stride;
+    const void* w;
+    int64_t w_stride;
+    const void* bias;
+    const void* residual;
+    int64_t residual_stride;
+    void* y;
+    int64_t y_stride;
+    void* saved;
+    void* values;
+    void* exponents;
+} tpb_layer;
+int tp_b200_layer_forward(const tpb_layer* layer, void* stream);
+
+/* Its gradients: dz (see tp_b200_activation_backward) from dy and what was
+ * saved -- either `saved`, contiguous, or values and exponents -- and from it
+ * dx [m, k] = dz w, dw [parts * n, k] = dz^T x (both contiguous), db [parts *
+ * n] = the column sums of dz before its rounding.  dx, dw, db may be NULL.
+ * dz: workspace [m, parts * n], row stride dz_stride; partial: workspace of
+ * groups * parts * n floats when db is wanted (1 <= groups <= 65535 groups of
+ * rows are summed apart, then joined in order). */
+typedef struct tpb_layer_grad {
+    int32_t dtype, act, parts, flags;
+    int64_t m, n, k, groups;
+    const void* dy;
+    int64_t dy_stride;
+    const void* x;
+    int64_t x_stride;
+    const void* w;
+    int64_t w_stride;
+    const void* saved;
+    const void* values;
+    const void* exponents;
+    void* dx;
+    void* dw;
+    void* db;
+    void* dz;
+    int64_t dz_stride;
+    float* partial;
+} tpb_layer_grad;
+int tp_b200_layer_backward(const tpb_layer_grad* grad, void* stream);
+
 /* y = act(z) [+ residual] for z [rows, n], y = act(z0) * z1 [+ residual] for
  * z [rows, 2, n]; y [rows, n] may be NULL.  values / exponents (may be NULL)
  * receive the checkpoint of z.  Rows may be strided; computed in fp32 and

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -74,6 +75,18 @@ def describe(t: torch.Tensor) -> TpbTensor:
         d.sizes[i] = s
         d.strides[i] = st
     return d
+
+
+# tpb_tensor, tpb_layer and tpb_layer_grad as packed bytes.
+_TENSOR = struct.Struct("Pii16q")
+LAYER = struct.Struct("4i3qPqPqPPqPqPPP")
+LAYER_GRAD = struct.Struct("4i4qPqPqPqPPPPPPPqP")
+
+
+def describe_rows(t: torch.Tensor, rows: int, n: int, pitch: int) -> TpbTensor:
+    """Descriptor of ``t``'s memory seen as [rows, n] with row stride ``pitch``."""
+    return TpbTensor.from_buffer_copy(_TENSOR.pack(t.data_ptr(), DTYPE_CODES[t.dtype], 2, rows, n, 0, 0, 0, 0, 0, 0,
+                                                   pitch, 1, 0, 0, 0, 0, 0, 0))
 
 
 _LOCK = threading.Lock()
@@ -143,8 +156,8 @@ _SIGNATURES = {
     "tp_b200_nll_loss_backward": ([_T, _T, _T, _T, _T, _I, _I64, _P], _I),
     "tp_b200_dropout": ([_T, _T, _T, _D, ctypes.c_uint64, ctypes.c_uint64, _P], _I),
     "tp_b200_masked_scale": ([_T, _T, _T, _D, _P], _I),
-    "tp_b200_linear_act": ([_T, _T, _T, _T, _T, _T, _T, _T, _I, _P], _I),
-    "tp_b200_gated_linear": ([_T, _T, _T, _T, _T, _T, _T, _I, _P], _I),
+    "tp_b200_layer_forward": ([_P, _P], _I),
+    "tp_b200_layer_backward": ([_P, _P], _I),
     "tp_b200_activation_forward": ([_T, _T, _T, _T, _T, _I, _P], _I),
     "tp_b200_activation_backward": ([_T, _T, _T, _T, _T, _T, _I, _P], _I),
     "tp_b200_checkpoint_unpack": ([_T, _T, _T, _P], _I),
@@ -209,4 +222,6 @@ def check(status: int, what: str = "") -> None:
 
 def stream_of(device: torch.device | int | None = None) -> int:
     """Handle of PyTorch's current stream on ``device`` (ordering matches torch)."""
+    if isinstance(device, torch.device) and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream

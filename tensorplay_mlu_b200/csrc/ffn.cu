@@ -8,6 +8,7 @@
 // results once.
 
 #include "act.cuh"
+#include "gemm.h"
 
 namespace tpb {
 namespace {
@@ -336,6 +337,31 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
     }
 }
 
+// out[c] = sum of partial[g][c] over the groups, in order: 32 columns a block,
+// its warps over the groups.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) column_sum_kernel(const float* __restrict__ partial, T* __restrict__ out,
+                                                              int groups, int64_t n) {
+    pdl_entry();
+    constexpr int kRows = kThreads / 32;
+    __shared__ float sums[kRows][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+    float s = 0.0f;
+    if (c < n) {
+#pragma unroll 4
+        for (int g = warp; g < groups; g += kRows) s += partial[int64_t(g) * n + c];
+    }
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < n) {
+        float total = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) total += sums[r][lane];
+        out[c] = store_as<T>(total);
+    }
+}
+
 void require_dtype(const tpb_tensor& t, int dtype, const char* what) {
     TPB_CHECK(t.dtype == dtype, "%s: expected %s, got %s", what, dtype_name(dtype), dtype_name(t.dtype));
 }
@@ -438,6 +464,32 @@ void dispatch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cuda
         if (vec) launch_backward<T, 8, GATED, false>(p, partial_rows, dev, s);
         else launch_backward<T, 1, GATED, false>(p, partial_rows, dev, s);
     }
+}
+
+void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t k, const char* what) {
+    TPB_CHECK(dtype == TPB_BF16 || dtype == TPB_F16 || dtype == TPB_F32,
+              "%s: expected bfloat16, float16 or float32, got %s", what, dtype_name(dtype));
+    require_act(act, what);
+    TPB_CHECK(parts == 1 || parts == 2, "%s: one part, or a gate and an up part; got %d", what, parts);
+    const int64_t limit = int64_t(1) << 30;
+    TPB_CHECK(m >= 0 && n >= 0 && k >= 0 && m < limit && n < limit && k < limit,
+              "%s: sizes %lld, %lld, %lld out of range", what, (long long)m, (long long)n, (long long)k);
+}
+
+GemmProblem product(int dtype, int64_t M, int64_t N, int64_t K, int flags) {
+    GemmProblem g{};
+    g.dtype = dtype;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.batch = 1;
+    g.alpha = 1.0;
+    g.flags = flags;
+    return g;
+}
+
+void run_gemm(const GemmProblem& p, int dev, cudaStream_t s) {
+    if (!gemm_tc(p, dev, s)) gemm_simt(p, dev, s);
 }
 
 #define TPB_DISPATCH_FFN(dtype, what, ...)                                        \
@@ -597,6 +649,190 @@ int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, con
             }
             check_launch("checkpoint_unpack");
         });
+    });
+}
+
+int tp_b200_layer_forward(const tpb_layer* a, void* stream) {
+    return guarded([&] {
+        TPB_CHECK(a != nullptr, "layer_forward: null arguments");
+        require_layer(a->dtype, a->act, a->parts, a->m, a->n, a->k, "layer_forward");
+        const int es = int(dtype_size(a->dtype));
+        const int64_t m = a->m, n = a->n, k = a->k;
+        TPB_CHECK((a->values == nullptr) == (a->exponents == nullptr), "layer_forward: a checkpoint is values and exponents");
+        if (m == 0 || n == 0) return;
+        const bool fused = a->dtype != TPB_F32 && k > 0;
+        TPB_CHECK(a->y != nullptr && (k == 0 || (a->x != nullptr && a->w != nullptr)), "layer_forward: null operand");
+        TPB_CHECK(a->parts == 1 || a->residual == nullptr, "layer_forward: the gated block takes no residual");
+        TPB_CHECK(fused || a->saved != nullptr, "layer_forward: float32, and no input features, need `saved`");
+        TPB_CHECK(!fused || (rows16(a->x, a->x_stride, es) && rows16(a->w, a->w_stride, es) && a->x_stride > 0 &&
+                             a->w_stride > 0),
+                  "layer_forward: the rows of the input and the weight must start on 16-byte boundaries");
+        const int dev = device_of(a->y);
+        DeviceGuard guard(dev);
+        cudaStream_t s = resolve_stream(stream, dev);
+        if (fused) {
+            FfnProblem q{};
+            q.dtype = a->dtype;
+            q.M = m;
+            q.N = n;
+            q.K = k;
+            q.parts = a->parts;
+            q.x = a->x;
+            q.sx_m = a->x_stride;
+            q.w = a->w;
+            q.sw_n = a->w_stride;
+            q.y = a->y;
+            q.sy_m = a->y_stride;
+            q.bias = a->bias;
+            q.residual = a->residual;
+            q.sres_m = a->residual_stride;
+            q.saved = a->saved;
+            q.values = static_cast<int8_t*>(a->values);
+            q.exponents = static_cast<uint8_t*>(a->exponents);
+            q.act = a->act;
+            TPB_CHECK(gemm_ffn(q, dev, s), "layer_forward: operands do not fit the tensor maps");
+            return;
+        }
+        // The product (bias as its addend) into `saved`, the rest elementwise.
+        GemmProblem g = product(a->dtype, m, a->parts * n, k, a->flags);
+        g.a = a->x;
+        g.sa_m = a->x_stride;
+        g.sa_k = 1;
+        g.b = a->w;
+        g.sb_k = 1;
+        g.sb_n = a->w_stride;
+        g.c = a->saved;
+        g.sc_m = a->parts * n;
+        if (a->bias != nullptr) {
+            g.cin = a->bias;
+            g.sci_n = 1;
+            g.beta = 1.0;
+        }
+        run_gemm(g, dev, s);
+        TPB_DISPATCH_FFN(a->dtype, "layer_forward", {
+            ForwardParams<scalar_t> p{};
+            p.z = static_cast<const scalar_t*>(a->saved);
+            p.sz_m = a->parts * n;
+            p.sz_p = n;
+            p.residual = static_cast<const scalar_t*>(a->residual);
+            p.sr_m = a->residual_stride;
+            p.y = static_cast<scalar_t*>(a->y);
+            p.sy_m = a->y_stride;
+            p.values = static_cast<int8_t*>(a->values);
+            p.exponents = static_cast<uint8_t*>(a->exponents);
+            p.n = n;
+            p.act = a->act;
+            p.units = make_units(m, n);
+            if (a->parts == 2) launch_forward<scalar_t, true>(p, s);
+            else launch_forward<scalar_t, false>(p, s);
+        });
+    });
+}
+
+int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
+    return guarded([&] {
+        TPB_CHECK(a != nullptr, "layer_backward: null arguments");
+        require_layer(a->dtype, a->act, a->parts, a->m, a->n, a->k, "layer_backward");
+        const int es = int(dtype_size(a->dtype));
+        const int64_t m = a->m, n = a->n, k = a->k, wide = a->parts * n;
+        TPB_CHECK((a->values == nullptr) == (a->exponents == nullptr), "layer_backward: a checkpoint is values and exponents");
+        TPB_CHECK(a->saved == nullptr || a->values == nullptr, "layer_backward: the pre-activations are given in one form");
+        TPB_CHECK(a->db == nullptr || (a->partial != nullptr && a->groups >= 1 && a->groups <= 65535),
+                  "layer_backward: db needs a workspace of 1 to 65535 groups");
+        if (m == 0 || n == 0) {
+            // Nothing was summed: the gradients are zero.
+            const void* any = a->dw != nullptr ? a->dw : a->db != nullptr ? a->db : a->dx;
+            if (any == nullptr) return;
+            const int dev = device_of(any);
+            DeviceGuard guard(dev);
+            cudaStream_t s = resolve_stream(stream, dev);
+            if (a->dx != nullptr && m * k > 0) TPB_CUDA(cudaMemsetAsync(a->dx, 0, size_t(m * k) * es, s));
+            if (a->dw != nullptr && wide * k > 0) TPB_CUDA(cudaMemsetAsync(a->dw, 0, size_t(wide * k) * es, s));
+            if (a->db != nullptr && wide > 0) TPB_CUDA(cudaMemsetAsync(a->db, 0, size_t(wide) * es, s));
+            return;
+        }
+        TPB_CHECK(a->dy != nullptr && a->dz != nullptr && (a->saved != nullptr || a->values != nullptr),
+                  "layer_backward: null operand");
+        TPB_CHECK(a->dz_stride >= wide, "layer_backward: the workspace's rows hold %lld elements, not %lld",
+                  (long long)a->dz_stride, (long long)wide);
+        TPB_CHECK(k == 0 || ((a->dx == nullptr || a->w != nullptr) && (a->dw == nullptr || a->x != nullptr)),
+                  "layer_backward: null operand");
+        const int dev = device_of(a->dz);
+        DeviceGuard guard(dev);
+        cudaStream_t s = resolve_stream(stream, dev);
+        TPB_DISPATCH_FFN(a->dtype, "layer_backward", {
+            BackwardParams<scalar_t> p{};
+            p.dy = static_cast<const scalar_t*>(a->dy);
+            p.sdy_m = a->dy_stride;
+            p.z = static_cast<const scalar_t*>(a->saved);
+            p.sz_m = wide;
+            p.sz_p = n;
+            p.values = static_cast<const int8_t*>(a->values);
+            p.exponents = static_cast<const uint8_t*>(a->exponents);
+            p.nb = (n + kCkptBlock - 1) / kCkptBlock;
+            p.dz = static_cast<scalar_t*>(a->dz);
+            p.sdz_m = a->dz_stride;
+            p.sdz_p = n;
+            p.partial = a->db != nullptr ? a->partial : nullptr;
+            p.m = m;
+            p.n = n;
+            p.act = a->act;
+            if (a->parts == 2) dispatch_backward<scalar_t, true>(p, a->groups, dev, s);
+            else dispatch_backward<scalar_t, false>(p, a->groups, dev, s);
+        });
+        if (a->db != nullptr) {
+            const unsigned grid = static_cast<unsigned>((wide + 31) / 32);
+            TPB_DISPATCH_FFN(a->dtype, "layer_backward", {
+                launch_pdl(column_sum_kernel<scalar_t>, grid, kThreads, 0, s, static_cast<const float*>(a->partial),
+                           static_cast<scalar_t*>(a->db), static_cast<int>(a->groups), wide);
+            });
+            check_launch("column_sum");
+        }
+        if (k == 0) return;
+        if (a->dx != nullptr) {
+            // dx = dz w, the weight read in place.
+            bool done = false;
+            if (a->dtype != TPB_F32) {
+                FfnProblem q{};
+                q.dtype = a->dtype;
+                q.M = m;
+                q.N = k;
+                q.K = wide;
+                q.parts = 1;
+                q.x = a->dz;
+                q.sx_m = a->dz_stride;
+                q.w = a->w;
+                q.sw_n = a->w_stride;
+                q.w_transposed = 1;
+                q.y = a->dx;
+                q.sy_m = k;
+                done = gemm_ffn(q, dev, s);
+            }
+            if (!done) {
+                GemmProblem g = product(a->dtype, m, k, wide, a->flags);
+                g.a = a->dz;
+                g.sa_m = a->dz_stride;
+                g.sa_k = 1;
+                g.b = a->w;
+                g.sb_k = a->w_stride;
+                g.sb_n = 1;
+                g.c = a->dx;
+                g.sc_m = k;
+                run_gemm(g, dev, s);
+            }
+        }
+        if (a->dw != nullptr) {
+            GemmProblem g = product(a->dtype, wide, k, m, a->flags);
+            g.a = a->dz;
+            g.sa_m = 1;
+            g.sa_k = a->dz_stride;
+            g.b = a->x;
+            g.sb_k = a->x_stride;
+            g.sb_n = 1;
+            g.c = a->dw;
+            g.sc_m = k;
+            run_gemm(g, dev, s);
+        }
     });
 }
 

@@ -145,105 +145,3 @@ extern "C" int tp_b200_gemm_epilogue(int epilogue, const tpb_tensor* out, const 
         }
     });
 }
-
-namespace {
-
-void require_matrix(const tpb_tensor* t, int dtype, int64_t rows, int64_t cols, const char* what) {
-    check_tensor(t, what);
-    TPB_CHECK(t->dtype == dtype, "%s: expected %s, got %s", what, dtype_name(dtype), dtype_name(t->dtype));
-    TPB_CHECK(t->ndim == 2 && t->sizes[0] == rows && t->sizes[1] == cols, "%s: expected [%lld, %lld]", what,
-              (long long)rows, (long long)cols);
-    TPB_CHECK(t->strides[1] == 1 || cols <= 1, "%s: needs unit column stride", what);
-}
-
-// [rows, n] (parts 1) or [rows, 2, n], contiguous.
-void require_wide(const tpb_tensor* t, int dtype, int64_t rows, int parts, int64_t n, const char* what) {
-    check_tensor(t, what);
-    TPB_CHECK(t->dtype == dtype, "%s: expected %s, got %s", what, dtype_name(dtype), dtype_name(t->dtype));
-    const int nd = parts == 2 ? 3 : 2;
-    TPB_CHECK(t->ndim == nd && t->sizes[0] == rows && t->sizes[nd - 1] == n && (parts == 1 || t->sizes[1] == 2),
-              "%s: expected [%lld, %s%lld]", what, (long long)rows, parts == 2 ? "2, " : "", (long long)n);
-    TPB_CHECK(is_contiguous(*t), "%s: must be contiguous", what);
-}
-
-int feed_forward(const char* what, int parts, const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
-                 const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w, const tpb_tensor* bias,
-                 const tpb_tensor* residual, int act, void* stream) {
-    return guarded([&] {
-        check_tensor(y, what);
-        check_tensor(x, what);
-        TPB_CHECK(y->dtype == TPB_BF16 || y->dtype == TPB_F16, "%s: expected bfloat16 or float16, got %s", what,
-                  dtype_name(y->dtype));
-        TPB_CHECK(act >= TPB_ACT_NONE && act <= TPB_ACT_SILU, "%s: unknown activation %d", what, act);
-        TPB_CHECK(y->ndim == 2 && x->ndim == 2, "%s: 2-d input and result", what);
-        FfnProblem q{};
-        q.dtype = y->dtype;
-        q.M = y->sizes[0];
-        q.N = y->sizes[1];
-        q.K = x->sizes[1];
-        q.parts = parts;
-        require_matrix(y, q.dtype, q.M, q.N, what);
-        require_matrix(x, q.dtype, q.M, q.K, what);
-        check_tensor(w, what);
-        TPB_CHECK(w->dtype == q.dtype && w->ndim == 2 && w->sizes[0] == parts * q.N && w->sizes[1] == q.K,
-                  "%s: expected a weight [%lld, %lld] of the result's dtype", what, (long long)(parts * q.N),
-                  (long long)q.K);
-        // A weight with unit stride along its rows instead is read in place
-        // where no epilogue is asked for (the input gradient dz W).
-        const bool unit_k = w->strides[1] == 1 || (q.K == 1 && w->strides[0] != 1);
-        q.w_transposed = !unit_k && w->strides[0] == 1 && parts == 1 && bias == nullptr && residual == nullptr &&
-                         saved == nullptr && values == nullptr && act == TPB_ACT_NONE;
-        TPB_CHECK(unit_k || q.w_transposed, "%s: the weight needs unit column stride", what);
-        TPB_CHECK(q.K > 0, "%s: needs at least one input feature", what);
-        if (bias != nullptr) {
-            check_tensor(bias, what);
-            TPB_CHECK(bias->dtype == q.dtype && bias->ndim == 1 && bias->sizes[0] == parts * q.N &&
-                          (bias->strides[0] == 1 || bias->sizes[0] <= 1),
-                      "%s: expected a contiguous bias of %lld elements", what, (long long)(parts * q.N));
-            q.bias = bias->data;
-        }
-        if (residual != nullptr) {
-            require_matrix(residual, q.dtype, q.M, q.N, what);
-            q.residual = residual->data;
-            q.sres_m = residual->strides[0];
-        }
-        TPB_CHECK((values == nullptr) == (exponents == nullptr), "%s: a checkpoint is values and exponents", what);
-        TPB_CHECK(saved == nullptr || values == nullptr, "%s: save the pre-activations in one form", what);
-        if (saved != nullptr) {
-            require_wide(saved, q.dtype, q.M, parts, q.N, what);
-            q.saved = saved->data;
-        }
-        if (values != nullptr) {
-            require_wide(values, TPB_I8, q.M, parts, q.N, what);
-            require_wide(exponents, TPB_U8, q.M, parts, (q.N + 31) / 32, what);
-            q.values = static_cast<int8_t*>(values->data);
-            q.exponents = static_cast<uint8_t*>(exponents->data);
-        }
-        if (q.M == 0 || q.N == 0) return;
-        q.x = x->data;
-        q.sx_m = x->strides[0];
-        q.w = w->data;
-        q.sw_n = w->strides[q.w_transposed ? 1 : 0];
-        q.y = y->data;
-        q.sy_m = y->strides[0];
-        q.act = act;
-        const int dev = device_of(y->data);
-        DeviceGuard guard(dev);
-        TPB_CHECK(gemm_ffn(q, dev, resolve_stream(stream, dev)),
-                  "%s: the input's and the weight's rows must start on 16-byte boundaries", what);
-    });
-}
-
-}  // namespace
-
-extern "C" int tp_b200_linear_act(const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
-                                  const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w,
-                                  const tpb_tensor* bias, const tpb_tensor* residual, int act, void* stream) {
-    return feed_forward("linear_act", 1, y, saved, values, exponents, x, w, bias, residual, act, stream);
-}
-
-extern "C" int tp_b200_gated_linear(const tpb_tensor* y, const tpb_tensor* saved, const tpb_tensor* values,
-                                    const tpb_tensor* exponents, const tpb_tensor* x, const tpb_tensor* w,
-                                    const tpb_tensor* bias, int act, void* stream) {
-    return feed_forward("gated_linear", 2, y, saved, values, exponents, x, w, bias, nullptr, act, stream);
-}

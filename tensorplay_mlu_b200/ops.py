@@ -1028,6 +1028,7 @@ def layer_norm(input, normalized_shape, weight=None, bias=None, eps: float = 1e-
 # an activation, mul and add), so they stand outside KERNELS.
 
 _FFN_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_BLOCK = N.CHECKPOINT_BLOCK
 
 
 def _activation_code(activation: str, what: str) -> int:
@@ -1041,60 +1042,67 @@ def _ffn_check(what: str, x, *others) -> None:
     """Device tensors on one device, in one supported dtype."""
     if not _is_device(x):
         _require_device(x)
-    if x.dtype not in _FFN_DTYPES:
-        raise RuntimeError(f"{what}: expected bfloat16, float16 or float32, got {x.dtype}")
+    dtype, device = x.dtype, x.device
+    if dtype not in _FFN_DTYPES:
+        raise RuntimeError(f"{what}: expected bfloat16, float16 or float32, got {dtype}")
     for t in others:
         if t is None:
             continue
-        _require_device(t)
-        if t.dtype != x.dtype:
-            raise RuntimeError(f"{what}: expected operands of one dtype, got {x.dtype} and {t.dtype}")
-        if t.device != x.device:
+        if not _is_device(t):
+            _require_device(t)
+        if t.dtype != dtype:
+            raise RuntimeError(f"{what}: expected operands of one dtype, got {dtype} and {t.dtype}")
+        if t.device != device:
             raise RuntimeError(f"{what}: operands are on different devices")
 
 
-def _rows(t: torch.Tensor, rows: int, n: int) -> torch.Tensor:
-    """``t`` seen as [rows, n] with unit column stride (rows may be strided; copied when they cannot be)."""
+def _rows(t: torch.Tensor, n: int):
+    """(tensor, row stride) of ``t`` seen as rows of n elements with unit column
+    stride: itself when it is a matrix of such rows or dense, else a dense copy.
+    Callers keep the tensor until the kernel has been launched."""
     if t.dim() == 2 and (t.stride(1) == 1 or n <= 1):
-        return t
-    return _dense(t).view(rows, n)
+        return t, t.stride(0)
+    return _dense(t), n
 
 
-def _product_rows(t: torch.Tensor) -> torch.Tensor:
-    """A 2-d operand of a tensor-core product: itself when its rows start on
-    16-byte boundaries (what a tensor-map load needs), otherwise a copy whose
+def _product_rows(t: torch.Tensor, pitch: int, rows: int, n: int):
+    """(tensor, row stride) of a product's operand: as given when its rows
+    start on the 16-byte boundaries a tensor-map load needs, else a copy whose
     rows do (one pass over it, instead of a product on the CUDA cores)."""
     per = 16 // t.element_size()
-    if (t.data_ptr() % 16 == 0 and t.stride(0) % per == 0 and t.stride(0) > 0) or t.numel() == 0:
-        return t
-    pitch = (t.shape[1] + per - 1) // per * per
-    out = _empty((t.shape[0], pitch), t.dtype, t.device)[:, :t.shape[1]]
-    N.check(_lib().tp_b200_copy(describe(out), describe(t), _stream(t)), "copy")
-    return out
+    if pitch % per == 0 and pitch > 0 and t.data_ptr() % 16 == 0:
+        return t, pitch
+    if rows == 0 or n == 0:
+        return t, per
+    aligned = (n + per - 1) // per * per
+    if rows == 1 and t.data_ptr() % 16 == 0:
+        return t, aligned  # there is no second row
+    out = t.new_empty((rows, aligned))
+    N.check(_lib().tp_b200_copy(N.describe_rows(out, rows, n, aligned), N.describe_rows(t, rows, n, pitch), _stream(t)),
+            "copy")
+    return out, aligned
 
 
 def _layer_operands(what: str, input, weight, bias, parts: int):
-    """(x [rows, K], rows, out features per part, leading shape) of a linear layer, checked."""
+    """(leading shape, rows, out features per part, input features) of a linear layer, checked."""
     _ffn_check(what, input, weight, bias)
     if input.dim() == 0 or weight.dim() != 2:
         raise RuntimeError(f"{what}: expected [..., K] input and 2-d weight, got {list(input.shape)} and "
                            f"{list(weight.shape)}")
-    k, out = input.shape[-1], weight.shape[0]
-    if weight.shape[1] != k:
-        raise RuntimeError(f"{what}: input features {k} do not match the weight's {weight.shape[1]}")
+    lead, k = input.shape[:-1], input.shape[-1]
+    out, wk = weight.shape
+    if wk != k:
+        raise RuntimeError(f"{what}: input features {k} do not match the weight's {wk}")
     if out % parts:
         raise RuntimeError(f"{what}: the weight needs an even number of rows (gate rows, then up rows), got {out}")
-    if bias is not None and list(bias.shape) != [out]:
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != out):
         raise RuntimeError(f"{what}: expected a bias of {out} elements, got {list(bias.shape)}")
-    lead = input.shape[:-1]
-    rows = math.prod(lead)
-    return _rows(input, rows, k), rows, out // parts, lead
+    return lead, lead[0] if len(lead) == 1 else math.prod(lead), out // parts, k
 
 
-def _checkpoint_empty(shape, device):
-    blocks = (shape[-1] + N.CHECKPOINT_BLOCK - 1) // N.CHECKPOINT_BLOCK
-    return (torch.empty(shape, dtype=torch.int8, device=device),
-            torch.empty((*shape[:-1], blocks), dtype=torch.uint8, device=device))
+def _checkpoint_empty(like, shape):
+    return (like.new_empty(shape, dtype=torch.int8),
+            like.new_empty((*shape[:-1], (shape[-1] + _BLOCK - 1) // _BLOCK), dtype=torch.uint8))
 
 
 def _checkpoint_check(what: str, values, exponents, shape, device) -> None:
@@ -1102,8 +1110,8 @@ def _checkpoint_check(what: str, values, exponents, shape, device) -> None:
     if values.dtype != torch.int8 or exponents.dtype != torch.uint8:
         raise RuntimeError(f"{what}: a checkpoint is int8 values and uint8 exponents, got {values.dtype} and "
                            f"{exponents.dtype}")
-    blocks = (shape[-1] + N.CHECKPOINT_BLOCK - 1) // N.CHECKPOINT_BLOCK if len(shape) else 0
-    if list(values.shape) != list(shape) or list(exponents.shape) != [*shape[:-1], blocks]:
+    blocks = (shape[-1] + _BLOCK - 1) // _BLOCK if len(shape) else 0
+    if tuple(values.shape) != tuple(shape) or tuple(exponents.shape) != (*shape[:-1], blocks):
         raise RuntimeError(f"{what}: a checkpoint of shape {list(shape)} has values of that shape and exponents "
                            f"{[*shape[:-1], blocks]}, got {list(values.shape)} and {list(exponents.shape)}")
     if values.device != device or exponents.device != device:
@@ -1122,14 +1130,16 @@ def checkpoint_pack(x):
     _ffn_check("checkpoint_pack", x)
     if x.dim() == 0:
         raise RuntimeError("checkpoint_pack: expected at least one dimension")
-    n = x.shape[-1]
-    values, exponents = _checkpoint_empty(tuple(x.shape), x.device)
-    if x.numel():
-        rows = x.numel() // n
-        x2 = _rows(x, rows, n)
+    values, exponents = _checkpoint_empty(x, tuple(x.shape))
+    numel = x.numel()
+    if numel:
+        n = x.shape[-1]
+        rows = numel // n
+        blocks = (n + _BLOCK - 1) // _BLOCK
+        x, pitch = _rows(x, n)
         N.check(_lib().tp_b200_activation_forward(
-            None, describe(values.view(rows, n)), describe(exponents.view(rows, -1)), describe(x2), None, 0, _stream(x)),
-            "checkpoint_pack")
+            None, N.describe_rows(values, rows, n, n), N.describe_rows(exponents, rows, blocks, blocks),
+            N.describe_rows(x, rows, n, pitch), None, 0, _stream(x)), "checkpoint_pack")
     return values, exponents
 
 
@@ -1141,14 +1151,17 @@ def checkpoint_unpack(values, exponents, dtype: torch.dtype):
         raise RuntimeError(f"checkpoint_unpack: expected bfloat16, float16 or float32, got {dtype}")
     if values.dim() == 0:
         raise RuntimeError("checkpoint_unpack: expected at least one dimension")
-    _checkpoint_check("checkpoint_unpack", values, exponents, tuple(values.shape), values.device)
-    out = _empty(values.shape, dtype, values.device)
-    if out.numel():
+    _checkpoint_check("checkpoint_unpack", values, exponents, values.shape, values.device)
+    out = values.new_empty(values.shape, dtype=dtype)
+    numel = out.numel()
+    if numel:
         n = values.shape[-1]
-        rows = out.numel() // n
-        values, exponents = _dense(values).view(rows, n), _dense(exponents).view(rows, -1)
-        N.check(_lib().tp_b200_checkpoint_unpack(describe(out.view(rows, n)), describe(values), describe(exponents),
-                                                 _stream(values)), "checkpoint_unpack")
+        rows = numel // n
+        blocks = (n + _BLOCK - 1) // _BLOCK
+        values, exponents = _dense(values), _dense(exponents)
+        N.check(_lib().tp_b200_checkpoint_unpack(
+            N.describe_rows(out, rows, n, n), N.describe_rows(values, rows, n, n),
+            N.describe_rows(exponents, rows, blocks, blocks), _stream(values)), "checkpoint_unpack")
     return out
 
 
@@ -1157,124 +1170,111 @@ def checkpoint_activation_backward(grad_output, values, exponents, activation: s
     what = "checkpoint_activation_backward"
     code = _activation_code(activation, what)
     _ffn_check(what, grad_output)
-    _checkpoint_check(what, values, exponents, tuple(grad_output.shape), grad_output.device)
+    _checkpoint_check(what, values, exponents, grad_output.shape, grad_output.device)
     if grad_output.dim() == 0:
         raise RuntimeError(f"{what}: expected at least one dimension")
-    out = _empty(grad_output.shape, grad_output.dtype, grad_output.device)
-    if out.numel():
+    out = grad_output.new_empty(grad_output.shape)
+    numel = out.numel()
+    if numel:
         n = out.shape[-1]
-        rows = out.numel() // n
-        dy = _rows(grad_output, rows, n)
-        values, exponents = _dense(values).view(rows, n), _dense(exponents).view(rows, -1)
-        N.check(_lib().tp_b200_activation_backward(describe(out.view(rows, n)), None, describe(dy), None, describe(values),
-                                                   describe(exponents), code, _stream(dy)), what)
+        rows = numel // n
+        blocks = (n + _BLOCK - 1) // _BLOCK
+        dy, pitch = _rows(grad_output, n)
+        values, exponents = _dense(values), _dense(exponents)
+        N.check(_lib().tp_b200_activation_backward(
+            N.describe_rows(out, rows, n, n), None, N.describe_rows(dy, rows, n, pitch), None,
+            N.describe_rows(values, rows, n, n), N.describe_rows(exponents, rows, blocks, blocks), code, _stream(dy)),
+            what)
     return out
 
 
 def _layer_forward(what: str, input, weight, bias, residual, activation, parts: int, save: bool, checkpoint: bool):
     code = _activation_code(activation, what)
-    x, rows, n, lead = _layer_operands(what, input, weight, bias, parts)
+    lead, rows, n, k = _layer_operands(what, input, weight, bias, parts)
+    dtype = input.dtype
+    sr = 0
     if residual is not None:
         _ffn_check(what, input, residual)
-        if list(residual.shape) != [*lead, n]:
+        if tuple(residual.shape) != (*lead, n):
             raise RuntimeError(f"{what}: expected a residual of the result's shape {[*lead, n]}, got "
                                f"{list(residual.shape)}")
-        residual = _rows(residual, rows, n)
-    dev = x.device
-    y = _empty((*lead, n), x.dtype, dev)
-    wide = (rows, 2, n) if parts == 2 else (rows, n)
+        residual, sr = _rows(residual, n)
+    y = input.new_empty((*lead, n))
+    wide = (*lead, 2, n) if parts == 2 else (*lead, n)
     values = exponents = None
     if checkpoint:
-        values, exponents = _checkpoint_empty(wide, dev)
-    z = _empty(wide, x.dtype, dev) if save and not checkpoint else None
-    if rows and n and x.dtype != torch.float32 and x.shape[1]:
-        # One kernel; the pre-activations stay on chip unless they are saved.
-        # (Copies made here are named: a descriptor does not keep its tensor alive.)
-        xp, wp = _product_rows(x), _product_rows(_rows(weight, parts * n, x.shape[1]))
-        bp = _dense(bias) if bias is not None else None
-        args = [describe(y.view(rows, n)), describe(z) if z is not None else None,
-                describe(values) if checkpoint else None, describe(exponents) if checkpoint else None,
-                describe(xp), describe(wp), describe(bp) if bp is not None else None]
-        if parts == 2:
-            status = _lib().tp_b200_gated_linear(*args, code, _stream(x))
-        else:
-            status = _lib().tp_b200_linear_act(*args, describe(residual) if residual is not None else None, code,
-                                               _stream(x))
-        N.check(status, what)
-    elif rows and n:
-        # float32 (whose products are several launches), or no input features.
-        if z is None:
-            z = _empty(wide, x.dtype, dev)
-        _gemm(z.view(rows, parts * n), _product_rows(x), _product_rows(weight).t(), bias, 1.0,
-              1.0 if bias is not None else 0.0)
-        N.check(_lib().tp_b200_activation_forward(
-            describe(y.view(rows, n)), describe(values) if checkpoint else None,
-            describe(exponents) if checkpoint else None, describe(z),
-            describe(residual) if residual is not None else None, code, _stream(x)), what)
-    if checkpoint:
-        saved = (values.view(*lead, *wide[1:]), exponents.view(*lead, *exponents.shape[1:]))
-    else:
-        saved = z.view(*lead, *wide[1:]) if save else None
-    return y, saved
+        values, exponents = _checkpoint_empty(input, wide)
+    # One kernel computes 16-bit layers; float32 products (several launches),
+    # and layers without input features, leave the pre-activations in memory.
+    fused = dtype != torch.float32 and k > 0
+    z = input.new_empty(wide) if (save and not checkpoint) or not fused else None
+    if rows and n:
+        x, sx = _rows(input, k)
+        w, sw = _rows(weight, k)
+        if fused:
+            x, sx = _product_rows(x, sx, rows, k)
+            w, sw = _product_rows(w, sw, parts * n, k)
+        if bias is not None:
+            bias = _dense(bias)
+        args = N.LAYER.pack(
+            N.DTYPE_CODES[dtype], code, parts, 0 if fused else _gemm_flags(dtype), rows, n, k, x.data_ptr(), sx,
+            w.data_ptr(), sw, bias.data_ptr() if bias is not None else 0,
+            residual.data_ptr() if residual is not None else 0, sr, y.data_ptr(), n,
+            z.data_ptr() if z is not None else 0, values.data_ptr() if checkpoint else 0,
+            exponents.data_ptr() if checkpoint else 0)
+        N.check(_lib().tp_b200_layer_forward(args, _stream(input)), what)
+    return y, (values, exponents) if checkpoint else z if save else None
 
 
 def _layer_backward(what: str, grad_output, input, weight, saved, activation, parts: int, output_mask):
     code = _activation_code(activation, what)
-    x, rows, n, lead = _layer_operands(what, input, weight, None, parts)
+    lead, rows, n, k = _layer_operands(what, input, weight, None, parts)
     _ffn_check(what, input, grad_output)
-    if list(grad_output.shape) != [*lead, n]:
+    dtype, out = input.dtype, parts * n
+    if tuple(grad_output.shape) != (*lead, n):
         raise RuntimeError(f"{what}: expected a gradient of shape {[*lead, n]}, got {list(grad_output.shape)}")
-    dy = _rows(grad_output, rows, n)
-    wide = (rows, 2, n) if parts == 2 else (rows, n)
-    shape = (*lead, *wide[1:])
+    wide = (*lead, 2, n) if parts == 2 else (*lead, n)
     z = values = exponents = None
     if isinstance(saved, (tuple, list)):
         if len(saved) != 2:
             raise RuntimeError(f"{what}: a checkpoint is (values, exponents)")
-        _checkpoint_check(what, saved[0], saved[1], shape, x.device)
-        values, exponents = (_dense(t).view(*wide[:-1], t.shape[-1]) for t in saved)
+        values, exponents = saved
+        _checkpoint_check(what, values, exponents, wide, input.device)
+        values, exponents = _dense(values), _dense(exponents)
     else:
         _ffn_check(what, input, saved)
-        if saved is None or list(saved.shape) != list(shape):
-            raise RuntimeError(f"{what}: expected saved pre-activations of shape {list(shape)}, got "
+        if saved is None or tuple(saved.shape) != wide:
+            raise RuntimeError(f"{what}: expected saved pre-activations of shape {list(wide)}, got "
                                f"{None if saved is None else list(saved.shape)}")
-        z = _dense(saved).view(wide)
-    mask = list(output_mask) + [True] * (3 - len(output_mask))
-    dev, out = x.device, parts * n
-    dx = _empty(input.shape, x.dtype, dev) if mask[0] else None
-    dw = _empty(weight.shape, x.dtype, dev) if mask[1] else None
-    db = None
-    if not (mask[0] or mask[1] or mask[2]):
+        z = _dense(saved)
+    want_x, want_w, want_b = (*output_mask, True, True, True)[:3]
+    dx = input.new_empty(input.shape) if want_x else None
+    dw = weight.new_empty(weight.shape) if want_w else None
+    db = weight.new_empty((out,)) if want_b else None
+    if not (want_x or want_w or want_b):
         return None, None, None
-    if out == 0 or rows == 0:
-        for t in (dx, dw):
-            if t is not None and t.numel():
-                fill_(t, 0)
-        if mask[2]:
-            db = zeros_like(_empty((out,), x.dtype, dev))
-        return dx, dw, db
-    # dz [rows, parts * n] with rows on 16-byte boundaries, as the two products read it.
-    per = 16 // x.element_size()
+    # Workspace: dz [rows, out] with rows on 16-byte boundaries, as the two
+    # products read it, then the bias gradient's partial sums (fp32).
+    per = 16 // input.element_size()
     pitch = (out + per - 1) // per * per
-    dz = _empty((rows, pitch), x.dtype, dev)[:, :out]
-    groups = min(max(rows // 16, 1), 128)
-    partial = _empty((groups, out), torch.float32, dev) if mask[2] else None
-    dzv = dz.unflatten(1, (2, n)) if parts == 2 else dz
-    N.check(_lib().tp_b200_activation_backward(
-        describe(dzv), describe(partial) if partial is not None else None, describe(dy),
-        describe(z) if z is not None else None, describe(values) if values is not None else None,
-        describe(exponents) if exponents is not None else None, code, _stream(x)), what)
-    if dx is not None and dx.numel():
-        wp = _product_rows(_rows(weight, out, weight.shape[1]))
-        if x.dtype != torch.float32:
-            N.check(_lib().tp_b200_linear_act(describe(dx.view(rows, weight.shape[1])), None, None, None, describe(dz),
-                                              describe(wp.t()), None, None, 0, _stream(x)), what)
-        else:
-            _gemm(dx.view(rows, weight.shape[1]), dz, wp)
-    if dw is not None and dw.numel():
-        _gemm(dw, dz.t(), _product_rows(x))
-    if mask[2]:
-        db = _reduce(N.SUM, partial, [0], False, x.dtype)
+    groups = min(max(rows // 16, 1), 128) if want_b else 0
+    work = input.new_empty((rows * pitch + groups * out * (4 // input.element_size()),))
+    dy, sdy = _rows(grad_output, n)
+    x, sx = _rows(input, k)
+    w, sw = _rows(weight, k)
+    if dtype != torch.float32:
+        if want_w:
+            x, sx = _product_rows(x, sx, rows, k)
+        if want_x:
+            w, sw = _product_rows(w, sw, out, k)
+    base = work.data_ptr()
+    args = N.LAYER_GRAD.pack(
+        N.DTYPE_CODES[dtype], code, parts, _gemm_flags(dtype), rows, n, k, groups, dy.data_ptr(), sdy, x.data_ptr(), sx,
+        w.data_ptr(), sw, z.data_ptr() if z is not None else 0, values.data_ptr() if values is not None else 0,
+        exponents.data_ptr() if values is not None else 0, dx.data_ptr() if want_x else 0,
+        dw.data_ptr() if want_w else 0, db.data_ptr() if want_b else 0, base, pitch,
+        base + rows * pitch * input.element_size() if want_b else 0)
+    N.check(_lib().tp_b200_layer_backward(args, _stream(input)), what)
     return dx, dw, db
 
 
