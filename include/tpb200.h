@@ -425,15 +425,16 @@ enum tpb_activation {
 /* A linear layer with its activation: parts 1: y [m, n] = act(x w^T + bias) +
  * residual, w [n, k]; parts 2, the gated block's first half: y = act(x wg^T +
  * bg) * (x wu^T + bu), w = [wg; wu] [2 n, k], bias [2 n], no residual.  Each
- * is one kernel for bfloat16 and float16: sums, bias, activation, gate and
- * residual in fp32, one rounding at the end.  Matrices have unit column
+ * is one kernel: sums, bias, activation, gate and residual in fp32, one
+ * rounding at the end.  Matrices have unit column
  * stride and the row strides given (elements); for bfloat16 and float16 the
  * rows of x and w start on 16-byte boundaries.
- *   saved       may be NULL: receives the pre-activations [m, n] / [m, 2, n].
- *               float32, and k = 0, need it (their product is written there).
+ *   saved       may be NULL: receives the pre-activations [m, n] / [m, 2, n]
+ *               (k = 0 needs it: the bias is written there).
  *   values, exponents   may be NULL: receive their 8-bit checkpoint.
  *   bias, residual      may be NULL.
- *   flags       as tp_b200_gemm (float32 products). */
+ *   flags       TPB_GEMM_ALLOW_TF32: float32 products may be one TF32 product;
+ *               otherwise they keep fp32 accuracy. */
 typedef struct tpb_layer {
     int32_t dtype, act, parts, flags;
     int64_t m, n, k;

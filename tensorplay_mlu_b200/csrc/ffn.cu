@@ -476,15 +476,24 @@ void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t 
               "%s: sizes %lld, %lld, %lld out of range", what, (long long)m, (long long)n, (long long)k);
 }
 
-GemmProblem product(int dtype, int64_t M, int64_t N, int64_t K, int flags) {
+// x w^T without an epilogue, for the plain products' kernels.
+GemmProblem plain_product(const FfnProblem& q) {
     GemmProblem g{};
-    g.dtype = dtype;
-    g.M = M;
-    g.N = N;
-    g.K = K;
+    g.dtype = q.dtype;
+    g.M = q.M;
+    g.N = q.N;
+    g.K = q.K;
     g.batch = 1;
+    g.a = q.x;
+    g.sa_m = q.sx_m;
+    g.sa_k = q.sx_k;
+    g.b = q.w;
+    g.sb_k = q.sw_k;
+    g.sb_n = q.sw_n;
+    g.c = q.y;
+    g.sc_m = q.sy_m;
     g.alpha = 1.0;
-    g.flags = flags;
+    g.flags = q.flags;
     return g;
 }
 
@@ -660,11 +669,11 @@ int tp_b200_layer_forward(const tpb_layer* a, void* stream) {
         const int64_t m = a->m, n = a->n, k = a->k;
         TPB_CHECK((a->values == nullptr) == (a->exponents == nullptr), "layer_forward: a checkpoint is values and exponents");
         if (m == 0 || n == 0) return;
-        const bool fused = a->dtype != TPB_F32 && k > 0;
+        const bool fused = k > 0;
         TPB_CHECK(a->y != nullptr && (k == 0 || (a->x != nullptr && a->w != nullptr)), "layer_forward: null operand");
         TPB_CHECK(a->parts == 1 || a->residual == nullptr, "layer_forward: the gated block takes no residual");
-        TPB_CHECK(fused || a->saved != nullptr, "layer_forward: float32, and no input features, need `saved`");
-        TPB_CHECK(!fused || (rows16(a->x, a->x_stride, es) && rows16(a->w, a->w_stride, es) && a->x_stride > 0 &&
+        TPB_CHECK(fused || a->saved != nullptr, "layer_forward: a layer without input features needs `saved`");
+        TPB_CHECK(!fused || a->dtype == TPB_F32 || (rows16(a->x, a->x_stride, es) && rows16(a->w, a->w_stride, es) && a->x_stride > 0 &&
                              a->w_stride > 0),
                   "layer_forward: the rows of the input and the weight must start on 16-byte boundaries");
         const int dev = device_of(a->y);
@@ -679,8 +688,11 @@ int tp_b200_layer_forward(const tpb_layer* a, void* stream) {
             q.parts = a->parts;
             q.x = a->x;
             q.sx_m = a->x_stride;
+            q.sx_k = 1;
             q.w = a->w;
             q.sw_n = a->w_stride;
+            q.sw_k = 1;
+            q.flags = a->flags;
             q.y = a->y;
             q.sy_m = a->y_stride;
             q.bias = a->bias;
@@ -690,17 +702,17 @@ int tp_b200_layer_forward(const tpb_layer* a, void* stream) {
             q.values = static_cast<int8_t*>(a->values);
             q.exponents = static_cast<uint8_t*>(a->exponents);
             q.act = a->act;
-            TPB_CHECK(gemm_ffn(q, dev, s), "layer_forward: operands do not fit the tensor maps");
+            if (a->dtype == TPB_F32) gemm_f32(q, dev, s);
+            else TPB_CHECK(gemm_ffn(q, dev, s), "layer_forward: operands do not fit the tensor maps");
             return;
         }
-        // The product (bias as its addend) into `saved`, the rest elementwise.
-        GemmProblem g = product(a->dtype, m, a->parts * n, k, a->flags);
-        g.a = a->x;
-        g.sa_m = a->x_stride;
-        g.sa_k = 1;
-        g.b = a->w;
-        g.sb_k = 1;
-        g.sb_n = a->w_stride;
+        // No input features: the bias is the pre-activation.
+        GemmProblem g{};
+        g.dtype = a->dtype;
+        g.M = m;
+        g.N = a->parts * n;
+        g.batch = 1;
+        g.a = g.b = a->saved;  // not read
         g.c = a->saved;
         g.sc_m = a->parts * n;
         if (a->bias != nullptr) {
@@ -708,7 +720,7 @@ int tp_b200_layer_forward(const tpb_layer* a, void* stream) {
             g.sci_n = 1;
             g.beta = 1.0;
         }
-        run_gemm(g, dev, s);
+        gemm_simt(g, dev, s);
         TPB_DISPATCH_FFN(a->dtype, "layer_forward", {
             ForwardParams<scalar_t> p{};
             p.z = static_cast<const scalar_t*>(a->saved);
@@ -789,49 +801,41 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             check_launch("column_sum");
         }
         if (k == 0) return;
+        FfnProblem q{};
+        q.dtype = a->dtype;
+        q.parts = 1;
+        q.flags = a->flags;
         if (a->dx != nullptr) {
             // dx = dz w, the weight read in place.
-            bool done = false;
-            if (a->dtype != TPB_F32) {
-                FfnProblem q{};
-                q.dtype = a->dtype;
-                q.M = m;
-                q.N = k;
-                q.K = wide;
-                q.parts = 1;
-                q.x = a->dz;
-                q.sx_m = a->dz_stride;
-                q.w = a->w;
-                q.sw_n = a->w_stride;
-                q.w_transposed = 1;
-                q.y = a->dx;
-                q.sy_m = k;
-                done = gemm_ffn(q, dev, s);
-            }
-            if (!done) {
-                GemmProblem g = product(a->dtype, m, k, wide, a->flags);
-                g.a = a->dz;
-                g.sa_m = a->dz_stride;
-                g.sa_k = 1;
-                g.b = a->w;
-                g.sb_k = a->w_stride;
-                g.sb_n = 1;
-                g.c = a->dx;
-                g.sc_m = k;
-                run_gemm(g, dev, s);
-            }
+            q.M = m;
+            q.N = k;
+            q.K = wide;
+            q.x = a->dz;
+            q.sx_m = a->dz_stride;
+            q.sx_k = 1;
+            q.w = a->w;
+            q.sw_n = 1;
+            q.sw_k = a->w_stride;
+            q.y = a->dx;
+            q.sy_m = k;
+            if (a->dtype == TPB_F32) gemm_f32(q, dev, s);
+            else if (!gemm_ffn(q, dev, s)) run_gemm(plain_product(q), dev, s);
         }
         if (a->dw != nullptr) {
-            GemmProblem g = product(a->dtype, wide, k, m, a->flags);
-            g.a = a->dz;
-            g.sa_m = 1;
-            g.sa_k = a->dz_stride;
-            g.b = a->x;
-            g.sb_k = a->x_stride;
-            g.sb_n = 1;
-            g.c = a->dw;
-            g.sc_m = k;
-            run_gemm(g, dev, s);
+            // dw = dz^T x: its rows are dz's columns, its columns x's.
+            q.M = wide;
+            q.N = k;
+            q.K = m;
+            q.x = a->dz;
+            q.sx_m = 1;
+            q.sx_k = a->dz_stride;
+            q.w = a->x;
+            q.sw_n = 1;
+            q.sw_k = a->x_stride;
+            q.y = a->dw;
+            q.sy_m = k;
+            if (a->dtype == TPB_F32) gemm_f32(q, dev, s);
+            else run_gemm(plain_product(q), dev, s);
         }
     });
 }

@@ -34,19 +34,18 @@ void gemm_simt(const GemmProblem& p, int dev, cudaStream_t stream);
 // (dtype, TMA alignment); nothing has been launched then.
 bool gemm_tc(const GemmProblem& p, int dev, cudaStream_t stream);
 
-// A feed-forward product (tp_b200_linear_act, tp_b200_gated_linear).  x [M, K]
-// and w [parts * N, K] with unit stride along K; parts 2: gate rows, then up
-// rows.  16-bit floats.
+// A feed-forward product (tp_b200_layer_forward and the products of
+// tp_b200_layer_backward): y = epilogue(x w^T), x [M, K] and w [parts * N, K];
+// parts 2: gate rows, then up rows.
 struct FfnProblem {
     int dtype;
     int64_t M, N, K;
     int parts;
-    const void* x;
-    int64_t sx_m;
-    const void* w;
-    int64_t sw_n;
-    int w_transposed;  // w is [K, N] with unit stride along N (parts 1)
-    void* y;  // [M, N]
+    const void* x;         // element (m, k) at x + m * sx_m + k * sx_k
+    int64_t sx_m, sx_k;
+    const void* w;         // element (n, k) at w + n * sw_n + k * sw_k
+    int64_t sw_n, sw_k;
+    void* y;               // [M, N], unit column stride
     int64_t sy_m;
     const void* bias;      // [parts * N] or null
     const void* residual;  // [M, N] or null
@@ -55,12 +54,16 @@ struct FfnProblem {
     int8_t* values;        // the same in 8 bits, or null
     uint8_t* exponents;
     int act;
+    int flags;
 };
 
-// False when x or w does not fit the tensor maps (rows off 16-byte
-// boundaries) or K is 0; nothing has been launched then.
+// 16-bit floats: sx_k 1; sw_k 1, or sw_n 1 without an epilogue.  False when x
+// or w does not fit the tensor maps (rows off 16-byte boundaries) or K is 0;
+// nothing has been launched then.
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream);
 // The same for few rows; x and w fit the tensor maps.
 void gemm_few(const FfnProblem& q, int dev, cudaStream_t stream);
+// float32: sx_k and sw_k 1, or sw_n 1, or sx_m and sw_n 1; K >= 1.
+void gemm_f32(const FfnProblem& q, int dev, cudaStream_t stream);
 
 }  // namespace tpb

@@ -24,25 +24,13 @@
 // Every wait is bounded as in gemm_tc.cu; all threads reach the cluster
 // barriers.  No TMA multicast is used.
 
-#include "act.cuh"
-#include "gemm_tc.cuh"
+#include "gemm_few.cuh"
 
 namespace tpb {
 namespace {
 
 constexpr int kFewThreads = 192;  // warp 0 TMA producer, 1 MMA issuer, 2-5 accumulator readers
 constexpr int kFewWarps = kFewThreads / 32;
-
-struct FewParams {
-    int M, N, K;       // rows of x; result columns of one part; contraction
-    int k_blocks;
-    int row_tiles;     // ceil(M / kNT)
-    uint32_t idesc;
-    void* y;
-    int64_t sy_m;
-    FfnParams ffn;
-    int* err;
-};
 
 template <int NT>
 struct FewShape {
@@ -65,104 +53,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-}
-
-template <int V>
-__device__ __forceinline__ void ld_cluster(uint32_t cluster_addr, float (&v)[V]) {
-    static_assert(V == 2 || V == 4, "8 or 16 bytes");
-    if constexpr (V == 4) {
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                     : "r"(cluster_addr)
-                     : "memory");
-    } else {
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(cluster_addr) : "memory");
-    }
-}
-
-// V consecutive elements of a row, vectorised where all of them exist on a
-// boundary of their size.
-template <typename T, int V>
-__device__ __forceinline__ void load_few(const T* src, int64_t left, float (&v)[V]) {
-    if (left >= V && reinterpret_cast<uintptr_t>(src) % (V * sizeof(T)) == 0) {
-        unpack_vec(*reinterpret_cast<const Vec<T, V>*>(src), v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < left ? load_as<float>(src[j]) : 0.0f;
-    }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_few(T* dst, int64_t left, const float (&v)[V]) {
-    if (left >= V && reinterpret_cast<uintptr_t>(dst) % (V * sizeof(T)) == 0) {
-        Vec<T, V> o;
-        pack_vec(v, o);
-        *reinterpret_cast<Vec<T, V>*>(dst) = o;
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if (j < left) dst[j] = store_as<T>(v[j]);
-        }
-    }
-}
-
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-    return r;
-}
-
-// V results of row m from column n on (a warp holds 32 V consecutive ones):
-// z[part] are their summed pre-activations.
-template <typename T, int PARTS, int V>
-__device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_t n, float (&z)[PARTS][V]) {
-    const FfnParams& f = p.ffn;
-    const int64_t left = p.N - n;  // may be negative
-    const T* bias = static_cast<const T*>(f.bias);
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
-        if (bias != nullptr && left > 0) {
-            float b[V];
-            load_few<T, V>(bias + int64_t(q) * p.N + n, left, b);
-#pragma unroll
-            for (int j = 0; j < V; ++j) z[q][j] += b[j];
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {  // rows of the weight past this part
-            if (j >= left) z[q][j] = 0.0f;
-        }
-        if (f.saved != nullptr && left > 0) {
-            store_few<T, V>(static_cast<T*>(f.saved) + m * f.ssaved_m + q * f.ssaved_p + n, left, z[q]);
-        }
-        if (f.values != nullptr) {
-            float amax = 0.0f;
-#pragma unroll
-            for (int j = 0; j < V; ++j) amax = max_nan(amax, fabsf(z[q][j]));
-#pragma unroll
-            for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            float qmax;
-            const int stored = ckpt_exponent<T>(amax, qmax);
-            const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
-            const int64_t row = m * PARTS + q;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (j < left) f.values[row * p.N + n + j] = ckpt_quantise(z[q][j], inverse, qmax);
-            }
-            if (n % kCkptBlock == 0 && left > 0) f.exponents[row * f.nb + n / kCkptBlock] = static_cast<uint8_t>(stored);
-        }
-    }
-    if (left <= 0) return;
-    act_values<true, V>(f.act, z[0]);
-    if constexpr (PARTS == 2) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) z[0][j] *= z[1][j];
-    }
-    if (f.residual != nullptr) {
-        float r[V];
-        load_few<T, V>(static_cast<const T*>(f.residual) + m * f.sres_m + n, left, r);
-#pragma unroll
-        for (int j = 0; j < V; ++j) z[0][j] += r[j];
-    }
-    store_few<T, V>(static_cast<T*>(p.y) + m * p.sy_m + n, left, z[0]);
 }
 
 template <typename T, int PARTS, int NT, bool W_MN>
@@ -294,37 +184,8 @@ __global__ void __launch_bounds__(kFewThreads)
     }
     __syncwarp();
     tc_fence_before();
-    cluster_sync();  // every CTA's partial sums are in its shared memory
-    tc_fence_after();
-    // partial[row of x][row of the weight tile]; a warp takes a row of x, a
-    // lane V columns of it, four ranks' loads in flight at a time.
-    constexpr int kV = kColumns / 32;
-    const int rows = min(NT, p.M - m0);
-    for (int m = rank + ranks * warp; m < rows; m += ranks * kFewWarps) {
-        float z[PARTS][kV];
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-            const uint32_t at = smem_addr(smem) + uint32_t(m * 128 + q * kColumns + lane * kV) * 4;
-#pragma unroll
-            for (int j = 0; j < kV; ++j) z[q][j] = 0.0f;
-            for (int c0 = 0; c0 < ranks; c0 += 4) {
-                float v[4][kV];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c0 + c < ranks) ld_cluster<kV>(map_to_cta(at, uint32_t(c0 + c)), v[c]);
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c0 + c < ranks) {
-#pragma unroll
-                        for (int j = 0; j < kV; ++j) z[q][j] += v[c][j];
-                    }
-                }
-            }
-        }
-        finish_few<T, PARTS, kV>(p, m0 + m, int64_t(n0) + lane * kV, z);
-    }
-    cluster_sync();  // no CTA leaves while another reads its shared memory
+    sum_and_finish<T, PARTS, NT>(p, reinterpret_cast<const float*>(smem), m0, n0, kFewWarps,
+                                 [](int64_t, int64_t, int, float&) {});
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -348,37 +209,8 @@ void launch_few(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType 
               (uint32_t(128 >> 4) << 24);
     p.row_tiles = (p.M + NT - 1) / NT;
     const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
-    // K's split: the cluster size with the fewest k-blocks in a row, a CTA's
-    // set-up and its share of the sum counted as eight of them.
-    const int64_t slots = int64_t(gemm_sm_budget(dev)) * S::kCtas;
-    int split = 1;
-    int64_t best = INT64_MAX;
-    for (int c = 1; c <= 8 && c <= p.k_blocks; ++c) {
-        const int64_t waves = (tiles * c + slots - 1) / slots;
-        const int64_t cost = waves * ((p.k_blocks + c - 1) / c + 8);
-        if (cost < best) {
-            best = cost;
-            split = c;
-        }
-    }
-    static const int forced = std::getenv("TPB200_FFN_SPLIT") ? std::atoi(std::getenv("TPB200_FFN_SPLIT")) : 0;
-    if (forced > 0) split = std::min(forced, p.k_blocks);
-    TPB_CHECK(tiles * split < (int64_t(1) << 31), "feed-forward product: too many tiles");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = static_cast<unsigned>(tiles * split);
-    cfg.blockDim = kFewThreads;
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    TPB_CUDA(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
+    p.split = choose_split(tiles, p.k_blocks, int64_t(num_sms(dev)) * S::kCtas, 8);
+    launch_cluster(kern, tiles * p.split, p.split, kFewThreads, S::kSmem, stream, mw, mx, p);
     check_launch("gemm_few");
 }
 
@@ -393,27 +225,9 @@ void launch_rows(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType
 
 template <typename T>
 void launch_typed(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream) {
-    FewParams p{};
-    p.M = static_cast<int>(q.M);
-    p.N = static_cast<int>(q.N);
-    p.K = static_cast<int>(q.K);
-    p.k_blocks = static_cast<int>((q.K + 63) / 64);
-    p.y = q.y;
-    p.sy_m = q.sy_m;
-    p.err = device_error_word(dev);
-    FfnParams& f = p.ffn;
-    f.bias = q.bias;
-    f.residual = q.residual;
-    f.sres_m = q.sres_m;
-    f.saved = q.saved;
-    f.ssaved_m = q.parts * q.N;
-    f.ssaved_p = q.N;
-    f.values = q.values;
-    f.exponents = q.exponents;
-    f.nb = (q.N + kCkptBlock - 1) / kCkptBlock;
-    f.act = q.act;
-    if (q.w_transposed) {
-        const CUtensorMap mw = make_map(q.w, type, 2, q.N, q.K, q.sw_n, 1, 0, 64);
+    FewParams p = few_params(q, dev, 64);
+    if (q.sw_k != 1) {
+        const CUtensorMap mw = make_map(q.w, type, 2, q.N, q.K, q.sw_k, 1, 0, 64);
         launch_rows<T, 1, true>(q, mw, type, p, dev, stream);
     } else {
         const CUtensorMap mw = make_map(q.w, type, 2, q.K, q.parts * q.N, q.sw_n, 1, 0, kBoxRows);

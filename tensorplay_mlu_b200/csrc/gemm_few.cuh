@@ -1,0 +1,233 @@
+// What the split-K feed-forward products share (gemm_few.cu for 16-bit floats,
+// gemm_f32.cu for float32): the sum of a cluster's partial accumulators over
+// distributed shared memory and the epilogue behind it.
+//
+// A tile is 128 rows of the weight -- the result's contiguous columns, so that
+// a warp stores whole segments of a row -- by kNT rows of x.  A gated tile is
+// 64 gate and 64 up rows of the weight.
+#pragma once
+
+#include "act.cuh"
+#include "gemm_tc.cuh"
+
+namespace tpb {
+namespace {
+
+struct FewParams {
+    int M, N, K;       // rows of x; result columns of one part; contraction
+    int k_blocks;
+    int row_tiles;     // ceil(M / kNT)
+    int split;         // CTAs of a cluster, which share K
+    uint32_t idesc;
+    void* y;
+    int64_t sy_m;
+    FfnParams ffn;
+    int* err;
+};
+
+template <int V>
+__device__ __forceinline__ void ld_cluster(uint32_t cluster_addr, float (&v)[V]) {
+    static_assert(V == 2 || V == 4, "8 or 16 bytes");
+    if constexpr (V == 4) {
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                     : "r"(cluster_addr)
+                     : "memory");
+    } else {
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(cluster_addr) : "memory");
+    }
+}
+
+// V consecutive elements of a row, vectorised where all of them exist on a
+// boundary of their size.
+template <typename T, int V>
+__device__ __forceinline__ void load_few(const T* src, int64_t left, float (&v)[V]) {
+    if (left >= V && reinterpret_cast<uintptr_t>(src) % (V * sizeof(T)) == 0) {
+        unpack_vec(*reinterpret_cast<const Vec<T, V>*>(src), v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = j < left ? load_as<float>(src[j]) : 0.0f;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_few(T* dst, int64_t left, const float (&v)[V]) {
+    if (left >= V && reinterpret_cast<uintptr_t>(dst) % (V * sizeof(T)) == 0) {
+        Vec<T, V> o;
+        pack_vec(v, o);
+        *reinterpret_cast<Vec<T, V>*>(dst) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (j < left) dst[j] = store_as<T>(v[j]);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+    return r;
+}
+
+// V results of row m from column n on (a warp holds 32 V consecutive ones):
+// z[part] are their summed pre-activations.
+template <typename T, int PARTS, int V>
+__device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_t n, float (&z)[PARTS][V]) {
+    const FfnParams& f = p.ffn;
+    const int64_t left = p.N - n;  // may be negative
+    const T* bias = static_cast<const T*>(f.bias);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+        if (bias != nullptr && left > 0) {
+            float b[V];
+            load_few<T, V>(bias + int64_t(q) * p.N + n, left, b);
+#pragma unroll
+            for (int j = 0; j < V; ++j) z[q][j] += b[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {  // rows of the weight past this part
+            if (j >= left) z[q][j] = 0.0f;
+        }
+        if (f.saved != nullptr && left > 0) {
+            store_few<T, V>(static_cast<T*>(f.saved) + m * f.ssaved_m + q * f.ssaved_p + n, left, z[q]);
+        }
+        if (f.values != nullptr) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) amax = max_nan(amax, fabsf(z[q][j]));
+#pragma unroll
+            for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            float qmax;
+            const int stored = ckpt_exponent<T>(amax, qmax);
+            const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+            const int64_t row = m * PARTS + q;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (j < left) f.values[row * p.N + n + j] = ckpt_quantise(z[q][j], inverse, qmax);
+            }
+            if (n % kCkptBlock == 0 && left > 0) f.exponents[row * f.nb + n / kCkptBlock] = static_cast<uint8_t>(stored);
+        }
+    }
+    if (left <= 0) return;
+    act_values<Narrow<T>::value, V>(f.act, z[0]);
+    if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[0][j] *= z[1][j];
+    }
+    if (f.residual != nullptr) {
+        float r[V];
+        load_few<T, V>(static_cast<const T*>(f.residual) + m * f.sres_m + n, left, r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[0][j] += r[j];
+    }
+    store_few<T, V>(static_cast<T*>(p.y) + m * p.sy_m + n, left, z[0]);
+}
+
+// The second half of a split-K tile.  partial: this CTA's sums, [row of x][row
+// of the weight tile], written before the call; every thread of every CTA of
+// the cluster calls it.  Each warp takes a row of x, each lane V columns of
+// it, four ranks' loads in flight at a time, added in rank order.
+// fix(row of x, result column, part, z): a chance to replace a sum.
+template <typename T, int PARTS, int NT, typename Fix>
+__device__ __forceinline__ void sum_and_finish(const FewParams& p, const float* partial, int m0, int n0, int warps,
+                                               Fix fix) {
+    constexpr int kColumns = 128 / PARTS;  // result columns of a tile
+    constexpr int kV = kColumns / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ranks = int(cluster_size());
+    const int rank = int(cluster_ctarank());
+    cluster_sync();  // every CTA's partial sums are in its shared memory
+    const int rows = min(NT, p.M - m0);
+    for (int m = rank + ranks * warp; m < rows; m += ranks * warps) {
+        float z[PARTS][kV];
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            const uint32_t at = smem_addr(partial) + uint32_t(m * 128 + q * kColumns + lane * kV) * 4;
+#pragma unroll
+            for (int j = 0; j < kV; ++j) z[q][j] = 0.0f;
+            for (int c0 = 0; c0 < ranks; c0 += 4) {
+                float v[4][kV];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c0 + c < ranks) ld_cluster<kV>(map_to_cta(at, uint32_t(c0 + c)), v[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c0 + c < ranks) {
+#pragma unroll
+                        for (int j = 0; j < kV; ++j) z[q][j] += v[c][j];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kV; ++j) fix(int64_t(m0) + m, int64_t(n0) + lane * kV + j, q, z[q][j]);
+        }
+        finish_few<T, PARTS, kV>(p, int64_t(m0) + m, int64_t(n0) + lane * kV, z);
+    }
+    cluster_sync();  // no CTA leaves while another reads its shared memory
+}
+
+// K's split: the cluster size with the fewest k-blocks in a row over `slots`
+// CTAs at a time, a CTA's set-up and its share of the sum counted as `fixed`
+// of them.
+inline int choose_split(int64_t tiles, int k_blocks, int64_t slots, int fixed) {
+    int split = 1;
+    int64_t best = INT64_MAX;
+    for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
+        const int64_t waves = (tiles * c + slots - 1) / slots;
+        const int64_t cost = waves * ((k_blocks + c - 1) / c + fixed);
+        if (cost < best) {
+            best = cost;
+            split = c;
+        }
+    }
+    return split;
+}
+
+template <typename K, typename... Args>
+void launch_cluster(K* kern, int64_t ctas, int cluster, int threads, size_t smem, cudaStream_t stream,
+                    const Args&... args) {
+    TPB_CHECK(ctas < (int64_t(1) << 31), "feed-forward product: too many tiles");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = static_cast<unsigned>(ctas);
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    TPB_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
+}
+
+// The operands of a problem's epilogue.
+inline FewParams few_params(const FfnProblem& q, int dev, int k_block) {
+    FewParams p{};
+    p.M = static_cast<int>(q.M);
+    p.N = static_cast<int>(q.N);
+    p.K = static_cast<int>(q.K);
+    p.k_blocks = static_cast<int>((q.K + k_block - 1) / k_block);
+    p.y = q.y;
+    p.sy_m = q.sy_m;
+    p.err = device_error_word(dev);
+    FfnParams& f = p.ffn;
+    f.bias = q.bias;
+    f.residual = q.residual;
+    f.sres_m = q.sres_m;
+    f.saved = q.saved;
+    f.ssaved_m = q.parts * q.N;
+    f.ssaved_p = q.N;
+    f.values = q.values;
+    f.exponents = q.exponents;
+    f.nb = (q.N + kCkptBlock - 1) / kCkptBlock;
+    f.act = q.act;
+    return p;
+}
+
+}  // namespace
+}  // namespace tpb

@@ -305,11 +305,12 @@ bool few_rows(const FfnProblem& q, int) {
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {
     const int64_t limit = int64_t(1) << 30;
     if (q.K == 0 || q.M >= limit || q.N >= limit || q.K >= limit) return false;
-    if (!tma_ok(q.x, 2, q.sx_m, 1, 0) || !tma_ok(q.w, 2, q.sw_n, 1, 0)) return false;
+    const bool transposed = q.sw_k != 1;
+    if (!tma_ok(q.x, 2, q.sx_m, 1, 0) || !tma_ok(q.w, 2, transposed ? q.sw_k : q.sw_n, 1, 0)) return false;
     TPB_CHECK(q.dtype == TPB_BF16 || q.dtype == TPB_F16, "feed-forward product: 16-bit floats only");
     if (few_rows(q, dev)) {
         gemm_few(q, dev, stream);
-    } else if (q.w_transposed) {
+    } else if (transposed) {
         // Without an epilogue this is the plain product.
         TPB_CHECK(q.bias == nullptr && q.residual == nullptr && q.saved == nullptr && q.values == nullptr &&
                       q.act == TPB_ACT_NONE,
@@ -324,7 +325,7 @@ bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {
         p.sa_m = q.sx_m;
         p.sa_k = 1;
         p.b = q.w;
-        p.sb_k = q.sw_n;
+        p.sb_k = q.sw_k;
         p.sb_n = 1;
         p.c = q.y;
         p.sc_m = q.sy_m;

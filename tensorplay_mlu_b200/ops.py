@@ -1204,20 +1204,19 @@ def _layer_forward(what: str, input, weight, bias, residual, activation, parts: 
     values = exponents = None
     if checkpoint:
         values, exponents = _checkpoint_empty(input, wide)
-    # One kernel computes 16-bit layers; float32 products (several launches),
-    # and layers without input features, leave the pre-activations in memory.
-    fused = dtype != torch.float32 and k > 0
-    z = input.new_empty(wide) if (save and not checkpoint) or not fused else None
+    # One kernel computes the layer; one without input features leaves its
+    # pre-activations (the bias) in memory.
+    z = input.new_empty(wide) if (save and not checkpoint) or k == 0 else None
     if rows and n:
         x, sx = _rows(input, k)
         w, sw = _rows(weight, k)
-        if fused:
+        if dtype != torch.float32 and k:
             x, sx = _product_rows(x, sx, rows, k)
             w, sw = _product_rows(w, sw, parts * n, k)
         if bias is not None:
             bias = _dense(bias)
         args = N.LAYER.pack(
-            N.DTYPE_CODES[dtype], code, parts, 0 if fused else _gemm_flags(dtype), rows, n, k, x.data_ptr(), sx,
+            N.DTYPE_CODES[dtype], code, parts, _gemm_flags(dtype), rows, n, k, x.data_ptr(), sx,
             w.data_ptr(), sw, bias.data_ptr() if bias is not None else 0,
             residual.data_ptr() if residual is not None else 0, sr, y.data_ptr(), n,
             z.data_ptr() if z is not None else 0, values.data_ptr() if checkpoint else 0,
