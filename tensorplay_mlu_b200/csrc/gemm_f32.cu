@@ -2,9 +2,9 @@
 // launch each: the forward layers with their epilogue, dz w and dz^T x.
 //
 // Every operand element is split on its way into shared memory, x = hi + lo
-// with hi = tf32(x) and lo = tf32(x - hi) (round to nearest), and a product is
-// hi hi + hi lo + lo hi: three TF32 MMAs.  The dropped lo lo and the rounding
-// of lo are 2^-22 of |a b|.  The tensor core rounds its running sum towards
+// with hi = x rounded to TF32 and lo = x - hi, read by the MMA as TF32 too, and
+// a product is hi hi + hi lo + lo hi: three TF32 MMAs.  The dropped lo lo and
+// lo's lost bits are at most 2^-21 of |a b|.  The tensor core rounds its running sum towards
 // zero, so a TMEM accumulator only takes kChain k-blocks (kChain * 32 terms);
 // warps of their own then add it to fp32 sums in registers, rounded to
 // nearest, while the MMAs fill the other accumulator.
@@ -36,7 +36,7 @@ struct F32Operands {
     int64_t sw_n, sw_k;
     const float* x;  // element (m, k) at x + m * sx_m + k * sx_k
     int64_t sx_m, sx_k;
-    int vec_w, vec_x;  // 16-byte loads along k
+    int vec_w, vec_x;  // 16-byte loads along the unit stride
     int tf32;          // one TF32 product is enough
 };
 
@@ -49,61 +49,135 @@ struct F32Shape {
     static constexpr int kAccWarps = NT == 128 ? 8 : 4;
     static constexpr int kAccCols = NT * 4 / kAccWarps;  // columns an accumulator warp sums
     static constexpr int kThreads = 32 * (kLoadWarps + 1 + kAccWarps);
-    static constexpr int kDepth = NT == 128 ? 2 : 3;  // k-blocks in registers
     static constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024 + 256;
-    static constexpr int kTmemCols = 2 * NT;
+    static constexpr int kTmemCols = 4 * NT;  // two accumulators: hi hi, and the cross terms
     static_assert(NT * 512 <= kStages * int(kStageBytes), "partial sums fit the stages");
 };
 
-// Four consecutive k of one row (zero outside).
-template <bool MN>
-__device__ __forceinline__ float4 load_chunk(const float* base, int64_t s_row, int64_t s_k, int64_t row, bool row_ok,
-                                             int k, int K, bool vec) {
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (!row_ok) return v;
-    if constexpr (MN) {
-        const float* p = base + row + int64_t(k) * s_k;
-        if (k < K) v.x = p[0];
-        if (k + 1 < K) v.y = p[s_k];
-        if (k + 2 < K) v.z = p[2 * s_k];
-        if (k + 3 < K) v.w = p[3 * s_k];
-    } else {
-        const float* p = base + row * s_row + k;
-        if (vec && k + 4 <= K) {
-            v = *reinterpret_cast<const float4*>(p);
-        } else {
-            if (k < K) v.x = p[0];
-            if (k + 1 < K) v.y = p[1];
-            if (k + 2 < K) v.z = p[2];
-            if (k + 3 < K) v.w = p[3];
-        }
-    }
+__device__ __forceinline__ float4 ldg128(const float* p) {
+    float4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "l"(p));
     return v;
 }
 
-__device__ __forceinline__ float tf32_of(float x) {
-    uint32_t u;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(u) : "f"(x));
-    return __uint_as_float(u & 0xffffe000u);
+// hi and lo of four consecutive k (chunk q) of row r into their swizzled
+// tiles.  hi is rounded to nearest, ties away; lo's low bits are the MMA's to
+// drop (2^-10 of lo).  An infinity keeps hi = inf and makes lo NaN, a NaN
+// makes lo NaN.
+__device__ __forceinline__ void store_split(uint8_t* hi_tile, uint32_t lo_offset, int r, int q, float4 v) {
+    uint8_t* at = hi_tile + r * 128 + ((q ^ (r & 7)) << 4);
+    const auto hi = [](float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); };
+    const float4 h = make_float4(hi(v.x), hi(v.y), hi(v.z), hi(v.w));
+    *reinterpret_cast<float4*>(at) = h;
+    *reinterpret_cast<float4*>(at + lo_offset) = make_float4(v.x - h.x, v.y - h.y, v.z - h.z, v.w - h.w);
 }
 
-// hi and lo of a chunk to row r, chunk q of their swizzled tiles.
-__device__ __forceinline__ void store_split(uint8_t* hi_tile, uint8_t* lo_tile, int r, int q, float4 v) {
-    const int at = r * 128 + ((q ^ (r & 7)) << 4);
-    const float4 h = make_float4(tf32_of(v.x), tf32_of(v.y), tf32_of(v.z), tf32_of(v.w));
-    *reinterpret_cast<float4*>(hi_tile + at) = h;
-    *reinterpret_cast<float4*>(lo_tile + at) =
-        make_float4(tf32_of(v.x - h.x), tf32_of(v.y - h.y), tf32_of(v.z - h.z), tf32_of(v.w - h.w));
-}
+// One operand's share of a loader thread: kRows rows by 32 k of a block.
+// Along k (MN false): chunk q of rows r0 + 32 i, eight lanes a row.  Along the
+// rows (MN true): rows r0 .. r0 + 3 at four k, transposed by the store; the
+// lanes are numbered so that eight neighbours store to distinct banks.
+template <bool MN, int kRows>
+struct Loader {
+    static constexpr int kRegs = MN ? 4 : kRows / 32;
+    const float* ptr[MN ? 1 : kRegs];
+    int64_t s_k;
+    int r0, q, K;
+    int rows;  // valid rows from r0 on (MN), a bit for each i (else)
+    bool vec, active;
+
+    // row_ptr(r): element (r, 0) of the tile's row r, null outside.
+    template <typename RowPtr>
+    __device__ __forceinline__ void init(int K_, int64_t s_k_, bool vec_, RowPtr row_ptr) {
+        K = K_;
+        s_k = s_k_;
+        vec = vec_;
+        rows = 0;
+        if constexpr (MN) {
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            constexpr int kGroups = kRows / 32;
+            active = warp < 2 * kGroups;
+            r0 = (warp % kGroups) * 32 + (((lane >> 3) << 1) | ((lane >> 2) & 1)) * 4;
+            q = (warp / kGroups) * 4 + (lane & 3);
+            ptr[0] = active ? row_ptr(r0) : nullptr;
+            if (ptr[0] != nullptr) {
+                rows = 1;
+#pragma unroll
+                for (int j = 1; j < 4; ++j) rows += row_ptr(r0 + j) == ptr[0] + j ? 1 : 0;
+            }
+        } else {
+            active = true;
+            q = threadIdx.x & 7;
+            r0 = threadIdx.x >> 3;
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) {
+                ptr[i] = row_ptr(r0 + 32 * i);
+                if (ptr[i] != nullptr) rows |= 1 << i;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void fetch(int kb, float4 (&reg)[kRegs]) const {
+        const int k = kb * 32 + q * 4;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) reg[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if constexpr (MN) {
+            if (rows == 0) return;
+            const float* p = ptr[0] + int64_t(k) * s_k;
+            if (vec && rows == 4 && k + 4 <= K) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) reg[e] = ldg128(p + e * s_k);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (k + e >= K) break;
+                    const float* pe = p + e * s_k;
+                    reg[e].x = pe[0];
+                    if (rows > 1) reg[e].y = pe[1];
+                    if (rows > 2) reg[e].z = pe[2];
+                    if (rows > 3) reg[e].w = pe[3];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) {
+                if (!((rows >> i) & 1)) continue;
+                const float* p = ptr[i] + k;
+                if (vec && k + 4 <= K) {
+                    reg[i] = ldg128(p);
+                } else {
+                    if (k < K) reg[i].x = p[0];
+                    if (k + 1 < K) reg[i].y = p[1];
+                    if (k + 2 < K) reg[i].z = p[2];
+                    if (k + 3 < K) reg[i].w = p[3];
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(uint8_t* tile, uint32_t lo_offset, const float4 (&reg)[kRegs]) const {
+        if constexpr (MN) {
+            if (!active) return;
+            store_split(tile, lo_offset, r0, q, make_float4(reg[0].x, reg[1].x, reg[2].x, reg[3].x));
+            store_split(tile, lo_offset, r0 + 1, q, make_float4(reg[0].y, reg[1].y, reg[2].y, reg[3].y));
+            store_split(tile, lo_offset, r0 + 2, q, make_float4(reg[0].z, reg[1].z, reg[2].z, reg[3].z));
+            store_split(tile, lo_offset, r0 + 3, q, make_float4(reg[0].w, reg[1].w, reg[2].w, reg[3].w));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) store_split(tile, lo_offset, r0 + 32 * i, q, reg[i]);
+        }
+    }
+};
 
 template <int PARTS, int NT, bool W_MN, bool X_MN>
 __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(const FewParams p, const F32Operands o) {
     using S = F32Shape<NT>;
     constexpr int kStages = S::kStages;
     constexpr int kColumns = 128 / PARTS;
-    constexpr int kWChunks = 128 * 8 / (kLoadWarps * 32);
-    constexpr int kXChunks = NT * 8 / (kLoadWarps * 32);
-    constexpr int kDepth = S::kDepth;
+    using LoadW = Loader<W_MN, 128>;
+    using LoadX = Loader<X_MN, NT>;
+    constexpr int kDepth = LoadW::kRegs + LoadX::kRegs > 6 ? 2 : 3;  // k-blocks in registers
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * S::kStageBytes);
@@ -148,28 +222,23 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
 
     if (warp < kLoadWarps) {
         // ------------------------------------------------- load and split --
-        float4 reg[kDepth][kWChunks + kXChunks];
-        const auto row_of = [](bool mn, int c, int rows) { return mn ? c % rows : c >> 3; };
-        const auto part_of = [](bool mn, int c, int rows) { return mn ? c / rows : c & 7; };
-        const auto fetch = [&](int kb, float4 (&r)[kWChunks + kXChunks]) {
-            if (kb >= kb1) return;
+        LoadW load_w;
+        LoadX load_x;
+        load_w.init(p.K, o.sw_k, o.vec_w != 0, [&](int r) -> const float* {
+            const int col = n0 + r % kColumns;
+            return col < p.N ? o.w + (col + int64_t(r / kColumns) * p.N) * o.sw_n : nullptr;
+        });
+        load_x.init(p.K, o.sx_k, o.vec_x != 0, [&](int r) -> const float* {
+            return m0 + r < p.M ? o.x + int64_t(m0 + r) * o.sx_m : nullptr;
+        });
+        float4 reg_w[kDepth][LoadW::kRegs], reg_x[kDepth][LoadX::kRegs];
 #pragma unroll
-            for (int i = 0; i < kWChunks; ++i) {
-                const int c = int(threadIdx.x) + i * kLoadWarps * 32;
-                const int row = row_of(W_MN, c, 128), q = part_of(W_MN, c, 128);
-                const int col = n0 + row % kColumns;
-                r[i] = load_chunk<W_MN>(o.w, o.sw_n, o.sw_k, col + int64_t(row / kColumns) * p.N, col < p.N,
-                                        kb * 32 + q * 4, p.K, o.vec_w);
+        for (int d = 0; d < kDepth - 1; ++d) {
+            if (kb0 + d < kb1) {
+                load_w.fetch(kb0 + d, reg_w[d]);
+                load_x.fetch(kb0 + d, reg_x[d]);
             }
-#pragma unroll
-            for (int i = 0; i < kXChunks; ++i) {
-                const int c = int(threadIdx.x) + i * kLoadWarps * 32;
-                const int row = m0 + row_of(X_MN, c, NT), q = part_of(X_MN, c, NT);
-                r[kWChunks + i] = load_chunk<X_MN>(o.x, o.sx_m, o.sx_k, row, row < p.M, kb * 32 + q * 4, p.K, o.vec_x);
-            }
-        };
-#pragma unroll
-        for (int d = 0; d < kDepth - 1; ++d) fetch(kb0 + d, reg[d]);
+        }
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -177,23 +246,17 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
 #pragma unroll
             for (int d = 0; d < kDepth; ++d) {
                 if (kb + d >= kb1 || !ok) break;
-                fetch(kb + d + kDepth - 1, reg[(d + kDepth - 1) % kDepth]);
+                if (kb + d + kDepth - 1 < kb1) {
+                    load_w.fetch(kb + d + kDepth - 1, reg_w[(d + kDepth - 1) % kDepth]);
+                    load_x.fetch(kb + d + kDepth - 1, reg_x[(d + kDepth - 1) % kDepth]);
+                }
                 int granted = 1;
                 if (lane == 0) granted = mbar_wait(smem_addr(&empty[stage]), phase ^ 1, abort_flag) ? 1 : 0;
                 ok = __shfl_sync(0xffffffffu, granted, 0) != 0;
                 if (!ok) break;
                 uint8_t* at = smem + stage * S::kStageBytes;
-#pragma unroll
-                for (int i = 0; i < kWChunks; ++i) {
-                    const int c = int(threadIdx.x) + i * kLoadWarps * 32;
-                    store_split(at, at + S::kWBytes, row_of(W_MN, c, 128), part_of(W_MN, c, 128), reg[d][i]);
-                }
-#pragma unroll
-                for (int i = 0; i < kXChunks; ++i) {
-                    const int c = int(threadIdx.x) + i * kLoadWarps * 32;
-                    store_split(at + 2 * S::kWBytes, at + 2 * S::kWBytes + S::kXBytes, row_of(X_MN, c, NT),
-                                part_of(X_MN, c, NT), reg[d][kWChunks + i]);
-                }
+                load_w.store(at, S::kWBytes, reg_w[d]);
+                load_x.store(at + 2 * S::kWBytes, S::kXBytes, reg_x[d]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_addr(&full[stage]));
@@ -207,6 +270,8 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
     } else if (warp == kLoadWarps) {
         // ------------------------------------------------------ MMA issuer --
         if (lane == 0) {
+            const uint64_t desc0 = sw128_desc(smem_addr(smem), 16, 1024);
+            const uint32_t wide = p.idesc + (uint32_t(NT >> 3) << 17);  // N = 2 NT
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -221,19 +286,26 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
                     break;
                 }
                 tc_fence_after();
-                const uint32_t w_hi = smem_addr(smem + stage * S::kStageBytes), w_lo = w_hi + S::kWBytes;
-                const uint32_t x_hi = w_lo + S::kWBytes, x_lo = x_hi + S::kXBytes;
-                const uint32_t d = tmem + acc * NT;
+                // Descriptors advance in 16-byte units of the address field.
+                const uint64_t w_hi = desc0 + uint32_t(stage) * (S::kStageBytes / 16), w_lo = w_hi + S::kWBytes / 16;
+                const uint64_t x_hi = w_lo + S::kWBytes / 16;  // x_lo behind it
+                const uint32_t d = tmem + acc * 2 * NT;
+                uint32_t more = i % kChain != 0 ? 1u : 0u;
+                if (o.tf32) {
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t wh = sw128_desc(w_hi + kk * 32, 16, 1024), xh = sw128_desc(x_hi + kk * 32, 16, 1024);
-                    uint32_t more = (i % kChain != 0 || kk > 0) ? 1u : 0u;
-                    if (!o.tf32) {  // the small terms first
-                        umma<true>(d, sw128_desc(w_lo + kk * 32, 16, 1024), xh, p.idesc, more);
-                        umma<true>(d, wh, sw128_desc(x_lo + kk * 32, 16, 1024), p.idesc, 1u);
+                    for (int kk = 0; kk < 4; ++kk) {
+                        umma<true>(d, w_hi + kk * 2, x_hi + kk * 2, p.idesc, more);
                         more = 1u;
                     }
-                    umma<true>(d, wh, xh, p.idesc, more);
+                } else {
+                    // One pass over w_hi gives hi hi (columns 0 .. NT - 1) and
+                    // hi lo (the next NT), which lo hi joins.
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        umma<true>(d, w_hi + kk * 2, x_hi + kk * 2, wide, more);
+                        more = 1u;
+                        umma<true>(d + NT, w_lo + kk * 2, x_hi + kk * 2, p.idesc, 1u);
+                    }
                 }
                 umma_commit(smem_addr(&empty[stage]));
                 if (i % kChain == kChain - 1 || i == kb1 - kb0 - 1) umma_commit(smem_addr(&acc_full[acc]));
@@ -262,13 +334,20 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
             ok = __shfl_sync(0xffffffffu, granted, 0) != 0;
             if (!ok) break;
             tc_fence_after();
+            const uint32_t at = tmem + (uint32_t(quad * 32) << 16) + acc * 2 * NT + col0;
 #pragma unroll
-            for (int c = 0; c < S::kAccCols; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(tmem + (uint32_t(quad * 32) << 16) + acc * NT + col0 + c, r);
+            for (int c = 0; c < S::kAccCols; c += 16) {
+                uint32_t r[16];
+                if (!o.tf32) {
+                    tmem_ld16(at + NT + c, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(r[j]);
+                }
+                tmem_ld16(at + c, r);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
+                for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(r[j]);
             }
             tc_fence_before();
             __syncwarp();
@@ -284,14 +363,18 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
     }
     __syncwarp();
     tc_fence_before();
-    sum_and_finish<float, PARTS, NT>(
-        p, reinterpret_cast<const float*>(smem), m0, n0, S::kThreads / 32, [&](int64_t m, int64_t n, int q, float& z) {
+    cluster_sync();  // every CTA's partial sums are in its shared memory
+    // A NaN sum is computed again as fp32 arithmetic would.
+    finish_rows<float, PARTS, NT>(
+        p, reinterpret_cast<const float*>(smem), m0, n0, warp, S::kThreads / 32, rank, ranks,
+        [&](int64_t m, int64_t n, int q, float& z) {
             if (z == z || n >= p.N) return;
             const float* w = o.w + (n + int64_t(q) * p.N) * o.sw_n;
             const float* x = o.x + m * o.sx_m;
             z = 0.0f;
-            for (int64_t k = 0; k < p.K; ++k) z = fmaf(w[k * o.sw_k], x[k * o.sx_k], z);
+            for (int64_t k = 0; k < p.K && z == z; ++k) z = fmaf(w[k * o.sw_k], x[k * o.sx_k], z);
         });
+    cluster_sync();  // no CTA leaves while another reads its shared memory
     if (warp == kLoadWarps) {
         __syncwarp();
         tc_fence_after();
@@ -311,8 +394,8 @@ void launch_f32(FewParams& p, const F32Operands& o, int dev, cudaStream_t stream
     p.idesc = (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(NT >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     p.row_tiles = (p.M + NT - 1) / NT;
     const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
-    p.split = choose_split(tiles, p.k_blocks, num_sms(dev), 16);
-    launch_cluster(kern, tiles * p.split, p.split, S::kThreads, S::kSmem, stream, p, o);
+    const int split = choose_split(tiles, p.k_blocks, num_sms(dev), 16, 16);
+    launch_cluster(kern, tiles * split, split, S::kThreads, S::kSmem, stream, p, o);
     check_launch("gemm_f32");
 }
 
@@ -325,7 +408,9 @@ void launch_rows(FewParams& p, const F32Operands& o, int dev, cudaStream_t strea
     else launch_f32<PARTS, 128, W_MN, X_MN>(p, o, dev, stream);
 }
 
-bool vectors(const float* p, int64_t s_row) { return aligned16(p) && s_row % 4 == 0; }
+// 16-byte loads: along k rows have to start on such boundaries, along the rows
+// every k.
+bool vectors(const float* p, int64_t stride) { return aligned16(p) && stride % 4 == 0; }
 
 }  // namespace
 
@@ -338,12 +423,12 @@ void gemm_f32(const FfnProblem& q, int dev, cudaStream_t stream) {
     o.x = static_cast<const float*>(q.x);
     o.sx_m = q.sx_m;
     o.sx_k = q.sx_k;
-    o.vec_w = vectors(o.w, o.sw_n);
-    o.vec_x = vectors(o.x, o.sx_m);
     o.tf32 = (q.flags & TPB_GEMM_ALLOW_TF32) != 0;
     // A layer reads w and x along k; dz w reads w along its rows' elements,
     // dz^T x both operands (w's strides are then both 1 when it has one column).
     const bool x_mn = q.sx_k != 1, w_mn = q.sw_k != 1 || x_mn;
+    o.vec_w = vectors(o.w, w_mn ? o.sw_k : o.sw_n);
+    o.vec_x = vectors(o.x, x_mn ? o.sx_k : o.sx_m);
     if (q.parts == 2) launch_rows<2, false, false>(p, o, dev, stream);
     else if (!w_mn) launch_rows<1, false, false>(p, o, dev, stream);
     else if (!x_mn) launch_rows<1, true, false>(p, o, dev, stream);

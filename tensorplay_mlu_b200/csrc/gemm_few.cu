@@ -45,16 +45,6 @@ struct FewShape {
     static constexpr int kTmemCols = NT < 32 ? 32 : NT;  // a power of two
 };
 
-// 32 lanes x 16 consecutive 32-bit columns of TMEM into 16 registers.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
-
 template <typename T, int PARTS, int NT, bool W_MN>
 __global__ void __launch_bounds__(kFewThreads)
     gemm_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const FewParams p) {
@@ -184,8 +174,10 @@ __global__ void __launch_bounds__(kFewThreads)
     }
     __syncwarp();
     tc_fence_before();
-    sum_and_finish<T, PARTS, NT>(p, reinterpret_cast<const float*>(smem), m0, n0, kFewWarps,
-                                 [](int64_t, int64_t, int, float&) {});
+    cluster_sync();  // every CTA's partial sums are in its shared memory
+    finish_rows<T, PARTS, NT>(p, reinterpret_cast<const float*>(smem), m0, n0, warp, kFewWarps, rank, ranks,
+                              [](int64_t, int64_t, int, float&) {});
+    cluster_sync();  // no CTA leaves while another reads its shared memory
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -209,8 +201,8 @@ void launch_few(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType 
               (uint32_t(128 >> 4) << 24);
     p.row_tiles = (p.M + NT - 1) / NT;
     const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
-    p.split = choose_split(tiles, p.k_blocks, int64_t(num_sms(dev)) * S::kCtas, 8);
-    launch_cluster(kern, tiles * p.split, p.split, kFewThreads, S::kSmem, stream, mw, mx, p);
+    const int split = choose_split(tiles, p.k_blocks, int64_t(num_sms(dev)) * S::kCtas, 8, 8);
+    launch_cluster(kern, tiles * split, split, kFewThreads, S::kSmem, stream, mw, mx, p);
     check_launch("gemm_few");
 }
 

@@ -13,11 +13,21 @@
 namespace tpb {
 namespace {
 
+// 32 lanes x 16 consecutive 32-bit columns of TMEM into 16 registers.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
 struct FewParams {
     int M, N, K;       // rows of x; result columns of one part; contraction
     int k_blocks;
     int row_tiles;     // ceil(M / kNT)
-    int split;         // CTAs of a cluster, which share K
+    int tiles;         // gemm_f32.cu: tiles of the whole product
     uint32_t idesc;
     void* y;
     int64_t sy_m;
@@ -123,21 +133,38 @@ __device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_
     store_few<T, V>(static_cast<T*>(p.y) + m * p.sy_m + n, left, z[0]);
 }
 
-// The second half of a split-K tile.  partial: this CTA's sums, [row of x][row
-// of the weight tile], written before the call; every thread of every CTA of
-// the cluster calls it.  Each warp takes a row of x, each lane V columns of
-// it, four ranks' loads in flight at a time, added in rank order.
-// fix(row of x, result column, part, z): a chance to replace a sum.
+// Sums a tile over the cluster's ranks and finishes it.  partial: a CTA's sums,
+// [row of x][row of the weight tile] floats at the same address in every
+// rank.  Warp `warp` of `warps` takes every warps-th row of x of this rank's
+// share, each lane V columns of it, four ranks' loads in flight at a time,
+// added in rank order.  fix(row of x, result column, part, z): a chance to
+// replace a sum.
 template <typename T, int PARTS, int NT, typename Fix>
-__device__ __forceinline__ void sum_and_finish(const FewParams& p, const float* partial, int m0, int n0, int warps,
-                                               Fix fix) {
+__device__ __forceinline__ void finish_rows(const FewParams& p, const float* partial, int m0, int n0, int warp,
+                                            int warps, int rank, int ranks, Fix fix) {
     constexpr int kColumns = 128 / PARTS;  // result columns of a tile
     constexpr int kV = kColumns / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ranks = int(cluster_size());
-    const int rank = int(cluster_ctarank());
-    cluster_sync();  // every CTA's partial sums are in its shared memory
+    const int lane = threadIdx.x & 31;
     const int rows = min(NT, p.M - m0);
+    const int64_t n = int64_t(n0) + lane * kV;
+    if (ranks == 1) {
+        // Two rows at a time: their reads and the stores behind them overlap.
+#pragma unroll 2
+        for (int m = warp; m < rows; m += warps) {
+            float z[PARTS][kV];
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                const Vec<float, kV> v = *reinterpret_cast<const Vec<float, kV>*>(partial + m * 128 + q * kColumns + lane * kV);
+#pragma unroll
+                for (int j = 0; j < kV; ++j) {
+                    z[q][j] = v.v[j];
+                    fix(int64_t(m0) + m, n + j, q, z[q][j]);
+                }
+            }
+            finish_few<T, PARTS, kV>(p, int64_t(m0) + m, n, z);
+        }
+        return;
+    }
     for (int m = rank + ranks * warp; m < rows; m += ranks * warps) {
         float z[PARTS][kV];
 #pragma unroll
@@ -160,22 +187,21 @@ __device__ __forceinline__ void sum_and_finish(const FewParams& p, const float* 
                 }
             }
 #pragma unroll
-            for (int j = 0; j < kV; ++j) fix(int64_t(m0) + m, int64_t(n0) + lane * kV + j, q, z[q][j]);
+            for (int j = 0; j < kV; ++j) fix(int64_t(m0) + m, n + j, q, z[q][j]);
         }
-        finish_few<T, PARTS, kV>(p, int64_t(m0) + m, int64_t(n0) + lane * kV, z);
+        finish_few<T, PARTS, kV>(p, int64_t(m0) + m, n, z);
     }
-    cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
 // K's split: the cluster size with the fewest k-blocks in a row over `slots`
 // CTAs at a time, a CTA's set-up and its share of the sum counted as `fixed`
-// of them.
-inline int choose_split(int64_t tiles, int k_blocks, int64_t slots, int fixed) {
+// of them (`whole` where K is not split).
+inline int choose_split(int64_t tiles, int k_blocks, int64_t slots, int fixed, int whole) {
     int split = 1;
     int64_t best = INT64_MAX;
     for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
         const int64_t waves = (tiles * c + slots - 1) / slots;
-        const int64_t cost = waves * ((k_blocks + c - 1) / c + fixed);
+        const int64_t cost = waves * ((k_blocks + c - 1) / c + (c == 1 ? whole : fixed));
         if (cost < best) {
             best = cost;
             split = c;
