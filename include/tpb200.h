@@ -426,9 +426,14 @@ enum tpb_activation {
  * residual, w [n, k]; parts 2, the gated block's first half: y = act(x wg^T +
  * bg) * (x wu^T + bu), w = [wg; wu] [2 n, k], bias [2 n], no residual.  Each
  * is one kernel: sums, bias, activation, gate and residual in fp32, one
- * rounding at the end.  Matrices have unit column
- * stride and the row strides given (elements); for bfloat16 and float16 the
- * rows of x and w start on 16-byte boundaries.
+ * rounding at the end.  Matrices have unit column stride and the row strides
+ * given (elements).
+ *   x_work, w_work   16-byte-aligned workspaces of m (parts * n) rows of k
+ *               elements rounded up to 16 bytes: x and w are copied there first
+ *               when their rows start off 16-byte boundaries.  bfloat16 and
+ *               float16 need them then; float32 reads rows anywhere, and takes
+ *               the copies only when given the workspaces (they pay where the
+ *               operand is read by many tiles).
  *   saved       may be NULL: receives the pre-activations [m, n] / [m, 2, n]
  *               (k = 0 needs it: the bias is written there).
  *   values, exponents   may be NULL: receive their 8-bit checkpoint.
@@ -450,6 +455,8 @@ typedef struct tpb_layer {
     void* saved;
     void* values;
     void* exponents;
+    void* x_work;
+    void* w_work;
 } tpb_layer;
 int tp_b200_layer_forward(const tpb_layer* layer, void* stream);
 
@@ -459,7 +466,7 @@ int tp_b200_layer_forward(const tpb_layer* layer, void* stream);
  * n] = the column sums of dz before its rounding.  dx, dw, db may be NULL.
  * dz: workspace [m, parts * n], row stride dz_stride; partial: workspace of
  * groups * parts * n floats when db is wanted (1 <= groups <= 65535 groups of
- * rows are summed apart, then joined in order). */
+ * rows are summed apart, then joined in order); x_work, w_work as above. */
 typedef struct tpb_layer_grad {
     int32_t dtype, act, parts, flags;
     int64_t m, n, k, groups;
@@ -478,6 +485,8 @@ typedef struct tpb_layer_grad {
     void* dz;
     int64_t dz_stride;
     float* partial;
+    void* x_work;
+    void* w_work;
 } tpb_layer_grad;
 int tp_b200_layer_backward(const tpb_layer_grad* grad, void* stream);
 

@@ -79,8 +79,8 @@ def describe(t: torch.Tensor) -> TpbTensor:
 
 # tpb_tensor, tpb_layer and tpb_layer_grad as packed bytes.
 _TENSOR = struct.Struct("Pii16q")
-LAYER = struct.Struct("4i3qPqPqPPqPqPPP")
-LAYER_GRAD = struct.Struct("4i4qPqPqPqPPPPPPPqP")
+LAYER = struct.Struct("4i3qPqPqPPqPqPPPPP")
+LAYER_GRAD = struct.Struct("4i4qPqPqPqPPPPPPPqPPP")
 
 
 def describe_rows(t: torch.Tensor, rows: int, n: int, pitch: int) -> TpbTensor:

@@ -337,6 +337,44 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
     }
 }
 
+// Rows off 16-byte boundaries copied to rows on them, for operands that
+// tensor maps or 16-byte loads read: a thread writes 16 bytes, from aligned
+// words shifted into place where all of them lie inside the row, element by
+// element at the row's ends.  E: 2- or 4-byte elements.
+template <typename E>
+__global__ void __launch_bounds__(kThreads) align_rows_kernel(E* __restrict__ dst, int64_t dst_pitch,
+                                                              const E* __restrict__ src, int64_t src_pitch, int64_t n,
+                                                              int64_t chunks, int64_t row_chunks, FastDiv div) {
+    pdl_entry();
+    constexpr int kPer = 16 / int(sizeof(E));
+    constexpr int kU = 4;
+    const int64_t first = int64_t(blockIdx.x) * kThreads * kU + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+        const int64_t i = first + int64_t(u) * kThreads;
+        if (i >= chunks) break;
+        const int64_t row = chunks <= 0xffffffffll ? int64_t(div.div(uint32_t(i))) : i / row_chunks;
+        const int64_t col = (i - row * row_chunks) * kPer;
+        const E* s = src + row * src_pitch + col;
+        Vec<E, kPer> out;
+        const bool odd = sizeof(E) == 2 && (reinterpret_cast<uintptr_t>(s) & 2) != 0;
+        if (col + kPer + 1 <= n && (!odd || col > 0)) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(odd ? s - 1 : s);
+            uint32_t v[5];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = w[j];
+            v[4] = odd ? w[4] : 0;
+            uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = odd ? __funnelshift_r(v[j], v[j + 1], 16) : v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) out.v[j] = col + j < n ? s[j] : E(0);
+        }
+        *reinterpret_cast<Vec<E, kPer>*>(dst + row * dst_pitch + col) = out;
+    }
+}
+
 // out[c] = sum of partial[g][c] over the groups, in order: 32 columns a block,
 // its warps over the groups.
 template <typename T>
@@ -474,6 +512,33 @@ void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t 
     const int64_t limit = int64_t(1) << 30;
     TPB_CHECK(m >= 0 && n >= 0 && k >= 0 && m < limit && n < limit && k < limit,
               "%s: sizes %lld, %lld, %lld out of range", what, (long long)m, (long long)n, (long long)k);
+}
+
+// An operand of a product, copied into `work` (rows of n elements rounded up
+// to 16 bytes) where its rows start off 16-byte boundaries.
+struct Aligned {
+    const void* data;
+    int64_t pitch;
+};
+Aligned align_rows(const void* src, int64_t pitch, int64_t rows, int64_t n, int es, void* work, const char* what,
+                   cudaStream_t s) {
+    const int64_t per = 16 / es, aligned = (n + per - 1) / per * per;
+    if (aligned16(src) && pitch > 0 && pitch % per == 0) return {src, pitch};
+    if (aligned16(src) && rows == 1) return {src, aligned};  // there is no second row
+    TPB_CHECK(work != nullptr && aligned16(work), "%s: rows off 16-byte boundaries need an aligned workspace", what);
+    const int64_t row_chunks = aligned / per, chunks = rows * row_chunks;
+    const int64_t blocks = (chunks + kThreads * 4 - 1) / (kThreads * 4);
+    TPB_CHECK(blocks < (int64_t(1) << 31), "%s: too many elements", what);
+    const FastDiv div(static_cast<uint32_t>(std::min<int64_t>(row_chunks, 0xffffffffll)));
+    if (es == 2) {
+        launch_pdl(align_rows_kernel<uint16_t>, unsigned(blocks), kThreads, 0, s, static_cast<uint16_t*>(work), aligned,
+                   static_cast<const uint16_t*>(src), pitch, n, chunks, row_chunks, div);
+    } else {
+        launch_pdl(align_rows_kernel<uint32_t>, unsigned(blocks), kThreads, 0, s, static_cast<uint32_t*>(work), aligned,
+                   static_cast<const uint32_t*>(src), pitch, n, chunks, row_chunks, div);
+    }
+    check_launch("align_rows");
+    return {work, aligned};
 }
 
 // x w^T without an epilogue, for the plain products' kernels.
@@ -673,24 +738,28 @@ int tp_b200_layer_forward(const tpb_layer* a, void* stream) {
         TPB_CHECK(a->y != nullptr && (k == 0 || (a->x != nullptr && a->w != nullptr)), "layer_forward: null operand");
         TPB_CHECK(a->parts == 1 || a->residual == nullptr, "layer_forward: the gated block takes no residual");
         TPB_CHECK(fused || a->saved != nullptr, "layer_forward: a layer without input features needs `saved`");
-        TPB_CHECK(!fused || a->dtype == TPB_F32 || (rows16(a->x, a->x_stride, es) && rows16(a->w, a->w_stride, es) && a->x_stride > 0 &&
-                             a->w_stride > 0),
-                  "layer_forward: the rows of the input and the weight must start on 16-byte boundaries");
         const int dev = device_of(a->y);
         DeviceGuard guard(dev);
         cudaStream_t s = resolve_stream(stream, dev);
         if (fused) {
+            Aligned x{a->x, a->x_stride}, w{a->w, a->w_stride};
+            // float32 operands are read with plain loads; only products that
+            // asked for the copies get them.
+            if (a->dtype != TPB_F32 || a->x_work != nullptr) x = align_rows(x.data, x.pitch, m, k, es, a->x_work, "layer_forward", s);
+            if (a->dtype != TPB_F32 || a->w_work != nullptr) {
+                w = align_rows(w.data, w.pitch, a->parts * n, k, es, a->w_work, "layer_forward", s);
+            }
             FfnProblem q{};
             q.dtype = a->dtype;
             q.M = m;
             q.N = n;
             q.K = k;
             q.parts = a->parts;
-            q.x = a->x;
-            q.sx_m = a->x_stride;
+            q.x = x.data;
+            q.sx_m = x.pitch;
             q.sx_k = 1;
-            q.w = a->w;
-            q.sw_n = a->w_stride;
+            q.w = w.data;
+            q.sw_n = w.pitch;
             q.sw_k = 1;
             q.flags = a->flags;
             q.y = a->y;
@@ -801,6 +870,13 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             check_launch("column_sum");
         }
         if (k == 0) return;
+        Aligned x{a->x, a->x_stride}, w{a->w, a->w_stride};
+        if (a->dw != nullptr && (a->dtype != TPB_F32 || a->x_work != nullptr)) {
+            x = align_rows(x.data, x.pitch, m, k, es, a->x_work, "layer_backward", s);
+        }
+        if (a->dx != nullptr && (a->dtype != TPB_F32 || a->w_work != nullptr)) {
+            w = align_rows(w.data, w.pitch, wide, k, es, a->w_work, "layer_backward", s);
+        }
         FfnProblem q{};
         q.dtype = a->dtype;
         q.parts = 1;
@@ -813,9 +889,9 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             q.x = a->dz;
             q.sx_m = a->dz_stride;
             q.sx_k = 1;
-            q.w = a->w;
+            q.w = w.data;
             q.sw_n = 1;
-            q.sw_k = a->w_stride;
+            q.sw_k = w.pitch;
             q.y = a->dx;
             q.sy_m = k;
             if (a->dtype == TPB_F32) gemm_f32(q, dev, s);
@@ -829,9 +905,9 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             q.x = a->dz;
             q.sx_m = 1;
             q.sx_k = a->dz_stride;
-            q.w = a->x;
+            q.w = x.data;
             q.sw_n = 1;
-            q.sw_k = a->x_stride;
+            q.sw_k = x.pitch;
             q.y = a->dw;
             q.sy_m = k;
             if (a->dtype == TPB_F32) gemm_f32(q, dev, s);

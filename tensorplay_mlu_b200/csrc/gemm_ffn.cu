@@ -23,36 +23,15 @@
 namespace tpb {
 namespace {
 
-// Byte of element (row r, column c) in a warp's 32 x 32 staging tile of
-// 16-bit elements (64-byte-swizzled rows) or bytes (32-byte-swizzled rows).
-__device__ __forceinline__ int stage_offset16(int r, int c) {
-    return r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2;
-}
-__device__ __forceinline__ int stage_offset8(int r, int c) {
-    return r * 32 + (((c >> 4) ^ ((r >> 2) & 1)) << 4) + (c & 15);
-}
-
-// A staged 32 x 32 tile to rows that TMA cannot store (off 16-byte
-// boundaries): a row at a time, one element a lane.
-template <typename T>
-__device__ __forceinline__ void store_staged_rows(const uint8_t* stage, int lane, T* dst, int64_t pitch, int64_t cols,
-                                                  int64_t rows) {
-    for (int r = 0; r < 32; ++r) {
-        if (r < rows && lane < cols) {
-            const int at = sizeof(T) == 1 ? stage_offset8(r, lane) : stage_offset16(r, lane);
-            dst[r * pitch + lane] = *reinterpret_cast<const T*>(stage + at);
-        }
-    }
-}
-
-// ... and the residual's rows into one.
+// The residual's rows, where 16-byte loads cannot read them, into a staging
+// tile.
 template <typename T>
 __device__ __forceinline__ void load_staged_rows(uint8_t* stage, int lane, const T* src, int64_t pitch, int64_t cols,
                                                  int64_t rows) {
 #pragma unroll 8
     for (int r = 0; r < 32; ++r) {
         const T v = r < rows && lane < cols ? src[r * pitch + lane] : T(0.0f);
-        *reinterpret_cast<T*>(stage + stage_offset16(r, lane)) = v;
+        *reinterpret_cast<T*>(stage + stage_offset(2, r, lane)) = v;
     }
 }
 
@@ -90,7 +69,7 @@ __device__ __forceinline__ uint8_t stage_checkpoint(uint8_t* stage, int lane, co
         Vec<int8_t, 16> q;
 #pragma unroll
         for (int j = 0; j < 16; ++j) q.v[j] = ckpt_quantise(z[h * 16 + j], inverse, qmax);
-        *reinterpret_cast<Vec<int8_t, 16>*>(stage + stage_offset8(lane, h * 16)) = q;
+        *reinterpret_cast<Vec<int8_t, 16>*>(stage + stage_offset(1, lane, h * 16)) = q;
     }
     return static_cast<uint8_t>(stored);
 }
@@ -207,7 +186,7 @@ __device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUten
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                    z[0][j] += load_as<float>(*reinterpret_cast<const T*>(stage + stage_offset16(lane, j)));
+                    z[0][j] += load_as<float>(*reinterpret_cast<const T*>(stage + stage_offset(2, lane, j)));
                 }
                 __syncwarp();
             }

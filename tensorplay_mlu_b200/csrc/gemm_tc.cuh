@@ -332,13 +332,54 @@ __device__ __forceinline__ void add_addend_chunk(const TcParams& p, const T* cro
     }
 }
 
+// One 32 x 32 chunk into a warp's staging tile, rows swizzled the way the C
+// tensor map expects (64-byte rows for 16-bit types, 128-byte for fp32), so
+// the 32 lanes' 16-byte writes hit distinct banks.
+template <typename T>
+__device__ __forceinline__ void stage_chunk(uint8_t* stage, int lane, const Vec<T, 32>& packed) {
+    constexpr int kRowBytes = 32 * int(sizeof(T));
+    constexpr int kVecs = kRowBytes / 16;
+    const uint4* src = reinterpret_cast<const uint4*>(&packed);
+    uint8_t* row = stage + lane * kRowBytes;
+#pragma unroll
+    for (int q = 0; q < kVecs; ++q) {
+        const int phys = kRowBytes == 64 ? (q ^ ((lane >> 1) & 3)) : (q ^ (lane & 7));
+        *reinterpret_cast<uint4*>(row + phys * 16) = src[q];
+    }
+}
+
+// Byte of element (row r, column c) in a warp's 32 x 32 staging tile of
+// elements of es bytes: rows of 32 es bytes, their 16-byte chunks swizzled as
+// the tensor maps of the stores expect.
+__device__ __forceinline__ int stage_offset(int es, int r, int c) {
+    if (es == 1) return r * 32 + (((c >> 4) ^ ((r >> 2) & 1)) << 4) + (c & 15);
+    if (es == 2) return r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2;
+    return r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4;
+}
+
+// A staged 32 x 32 tile to rows that TMA cannot store (off 16-byte
+// boundaries): a row at a time, one element a lane.
+template <typename T>
+__device__ __forceinline__ void store_staged_rows(const uint8_t* stage, int lane, T* dst, int64_t pitch, int64_t cols,
+                                                  int64_t rows) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+        if (r < rows && lane < cols) {
+            dst[r * pitch + lane] = *reinterpret_cast<const T*>(stage + stage_offset(sizeof(T), r, lane));
+        }
+    }
+}
+
 // The epilogue of one accumulator: this warp's 32 rows (its TMEM lane
 // quadrant, t_rows = TMEM address of row 0 / column 0 of the accumulator)
 // for columns [col0, col0 + NCOL).  The load of chunk c + 1 is issued before
 // chunk c is converted and stored, so TMEM reads overlap the global stores.
+// Rows that allow no 16-byte stores go through the warp's staging tile, so that
+// 32 lanes store 32 neighbouring elements of a row (a row each, one element
+// at a time, wrote 32 sectors per instruction).
 template <typename T, int NCOL>
-__device__ __forceinline__ void store_accumulator(const TcParams& p, uint32_t t_rows, int col0, int b, int64_t gm,
-                                                  int64_t n_tile0, bool row_ok) {
+__device__ __forceinline__ void store_accumulator(const TcParams& p, uint8_t* stage, uint32_t t_rows, int col0, int b,
+                                                  int64_t gm, int64_t n_tile0, bool row_ok) {
     constexpr int kChunks = NCOL / 32;
     T* crow = static_cast<T*>(p.c) + b * p.sc_b + gm * p.sc_m;
     const T* cin = static_cast<const T*>(p.cin);
@@ -351,12 +392,22 @@ __device__ __forceinline__ void store_accumulator(const TcParams& p, uint32_t t_
         if (chunk + 1 < kChunks) tmem_ld32(t_rows + col0 + (chunk + 1) * 32, r[(chunk + 1) & 1]);
         const uint32_t* rc = r[chunk & 1];
         const int64_t n_base = n_tile0 + col0 + chunk * 32;
-        if (row_ok && n_base < p.N) {
+        if (n_base >= p.N) continue;
+        if (row_ok || !p.vec_store) {
             float v[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = p.alpha * __uint_as_float(rc[j]);
-            if (cin != nullptr) add_addend_chunk<T>(p, cin + b * p.sci_b + gm * p.sci_m, n_base, v);
-            if (p.vec_store && n_base + 32 <= p.N) {
+            if (cin != nullptr && row_ok) add_addend_chunk<T>(p, cin + b * p.sci_b + gm * p.sci_m, n_base, v);
+            if (!p.vec_store) {
+                const int lane = threadIdx.x & 31;
+                Vec<T, 32> packed;
+                pack_vec(v, packed);
+                __syncwarp();
+                stage_chunk<T>(stage, lane, packed);
+                __syncwarp();
+                store_staged_rows<T>(stage, lane, static_cast<T*>(p.c) + b * p.sc_b + (gm - lane) * p.sc_m + n_base,
+                                     p.sc_m, p.N - n_base, p.M - (gm - lane));
+            } else if (n_base + 32 <= p.N) {
                 constexpr int V = 16 / sizeof(T);
 #pragma unroll
                 for (int j = 0; j < 32; j += V) {
@@ -410,22 +461,6 @@ __device__ __forceinline__ float2 gelu_backward_narrow2(float2 dy, float2 z) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
     const float2 u = __fmul2_rn(z, f2(0.39894228040143267794f));
     return __fmul2_rn(dy, __ffma2_rn(u, e, phi_narrow2(z)));
-}
-
-// One 32 x 32 chunk into a warp's staging tile, rows swizzled the way the C
-// tensor map expects (64-byte rows for 16-bit types, 128-byte for fp32), so
-// the 32 lanes' 16-byte writes hit distinct banks.
-template <typename T>
-__device__ __forceinline__ void stage_chunk(uint8_t* stage, int lane, const Vec<T, 32>& packed) {
-    constexpr int kRowBytes = 32 * int(sizeof(T));
-    constexpr int kVecs = kRowBytes / 16;
-    const uint4* src = reinterpret_cast<const uint4*>(&packed);
-    uint8_t* row = stage + lane * kRowBytes;
-#pragma unroll
-    for (int q = 0; q < kVecs; ++q) {
-        const int phys = kRowBytes == 64 ? (q ^ ((lane >> 1) & 3)) : (q ^ (lane & 7));
-        *reinterpret_cast<uint4*>(row + phys * 16) = src[q];
-    }
 }
 
 // The same through shared memory and a TMA store: each chunk of 32 rows x
@@ -989,8 +1024,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTc2Threads, 1)
                                                                     gm, gm - lane, int64_t(nt) * kPairBN, gm < p.M,
                                                                     &tmAux, stage + staging_bytes<T>());
             } else {
-                store_accumulator<T, kPairBN / 2>(p, t_rows, half * (kPairBN / 2), b, gm, int64_t(nt) * kPairBN,
-                                                  gm < p.M);
+                store_accumulator<T, kPairBN / 2>(p, staging + (warp - 2) * staging_tiles<EPI>() * staging_bytes<T>(),
+                                                  t_rows, half * (kPairBN / 2), b, gm, int64_t(nt) * kPairBN, gm < p.M);
             }
             tc_fence_before();
             __syncwarp();

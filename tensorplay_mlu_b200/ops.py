@@ -1065,22 +1065,17 @@ def _rows(t: torch.Tensor, n: int):
     return _dense(t), n
 
 
-def _product_rows(t: torch.Tensor, pitch: int, rows: int, n: int):
-    """(tensor, row stride) of a product's operand: as given when its rows
-    start on the 16-byte boundaries a tensor-map load needs, else a copy whose
-    rows do (one pass over it, instead of a product on the CUDA cores)."""
+def _align_elements(t: torch.Tensor, pitch: int, rows: int, n: int, reads: int) -> int:
+    """Workspace elements for a product's operand: none when its rows start on
+    the 16-byte boundaries its loads need, else a copy whose rows do.  float32
+    products read rows anywhere, four times slower: they take the copy, one
+    pass over the operand, where at least four tiles read it."""
     per = 16 // t.element_size()
-    if pitch % per == 0 and pitch > 0 and t.data_ptr() % 16 == 0:
-        return t, pitch
-    if rows == 0 or n == 0:
-        return t, per
-    aligned = (n + per - 1) // per * per
-    if rows == 1 and t.data_ptr() % 16 == 0:
-        return t, aligned  # there is no second row
-    out = t.new_empty((rows, aligned))
-    N.check(_lib().tp_b200_copy(N.describe_rows(out, rows, n, aligned), N.describe_rows(t, rows, n, pitch), _stream(t)),
-            "copy")
-    return out, aligned
+    if (pitch % per == 0 and pitch > 0 or rows == 1) and t.data_ptr() % 16 == 0:
+        return 0
+    if t.dtype == torch.float32 and reads < 4:
+        return 0
+    return rows * ((n + per - 1) // per * per)
 
 
 def _layer_operands(what: str, input, weight, bias, parts: int):
@@ -1210,9 +1205,12 @@ def _layer_forward(what: str, input, weight, bias, residual, activation, parts: 
     if rows and n:
         x, sx = _rows(input, k)
         w, sw = _rows(weight, k)
-        if dtype != torch.float32 and k:
-            x, sx = _product_rows(x, sx, rows, k)
-            w, sw = _product_rows(w, sw, parts * n, k)
+        ex = _align_elements(x, sx, rows, k, n // 128) if k else 0
+        ew = _align_elements(w, sw, parts * n, k, rows // 64) if k else 0
+        xw = ww = 0
+        if ex or ew:
+            work = input.new_empty((ex + ew,))
+            xw, ww = work.data_ptr() if ex else 0, work.data_ptr() + ex * work.element_size() if ew else 0
         if bias is not None:
             bias = _dense(bias)
         args = N.LAYER.pack(
@@ -1220,7 +1218,7 @@ def _layer_forward(what: str, input, weight, bias, residual, activation, parts: 
             w.data_ptr(), sw, bias.data_ptr() if bias is not None else 0,
             residual.data_ptr() if residual is not None else 0, sr, y.data_ptr(), n,
             z.data_ptr() if z is not None else 0, values.data_ptr() if checkpoint else 0,
-            exponents.data_ptr() if checkpoint else 0)
+            exponents.data_ptr() if checkpoint else 0, xw, ww)
         N.check(_lib().tp_b200_layer_forward(args, _stream(input)), what)
     return y, (values, exponents) if checkpoint else z if save else None
 
@@ -1253,26 +1251,28 @@ def _layer_backward(what: str, grad_output, input, weight, saved, activation, pa
     if not (want_x or want_w or want_b):
         return None, None, None
     # Workspace: dz [rows, out] with rows on 16-byte boundaries, as the two
-    # products read it, then the bias gradient's partial sums (fp32).
+    # products read it, the bias gradient's partial sums (fp32), and copies of
+    # operands whose rows start elsewhere.
     per = 16 // input.element_size()
     pitch = (out + per - 1) // per * per
     groups = min(max(rows // 16, 1), 128) if want_b else 0
-    work = input.new_empty((rows * pitch + groups * out * (4 // input.element_size()),))
     dy, sdy = _rows(grad_output, n)
     x, sx = _rows(input, k)
     w, sw = _rows(weight, k)
-    if dtype != torch.float32:
-        if want_w:
-            x, sx = _product_rows(x, sx, rows, k)
-        if want_x:
-            w, sw = _product_rows(w, sw, out, k)
+    ex = _align_elements(x, sx, rows, k, out // 64) if want_w and k else 0
+    ew = _align_elements(w, sw, out, k, rows // 64) if want_x and k else 0
+    es = input.element_size()
+    sums = (groups * out * (4 // es) + per - 1) // per * per
+    work = input.new_empty((rows * pitch + sums + ex + ew,))
     base = work.data_ptr()
+    part = base + rows * pitch * es
+    xw = part + sums * es
     args = N.LAYER_GRAD.pack(
         N.DTYPE_CODES[dtype], code, parts, _gemm_flags(dtype), rows, n, k, groups, dy.data_ptr(), sdy, x.data_ptr(), sx,
         w.data_ptr(), sw, z.data_ptr() if z is not None else 0, values.data_ptr() if values is not None else 0,
         exponents.data_ptr() if values is not None else 0, dx.data_ptr() if want_x else 0,
-        dw.data_ptr() if want_w else 0, db.data_ptr() if want_b else 0, base, pitch,
-        base + rows * pitch * input.element_size() if want_b else 0)
+        dw.data_ptr() if want_w else 0, db.data_ptr() if want_b else 0, base, pitch, part if want_b else 0,
+        xw if ex else 0, xw + ex * es if ew else 0)
     N.check(_lib().tp_b200_layer_backward(args, _stream(input)), what)
     return dx, dw, db
 
