@@ -63,6 +63,7 @@ struct FfnProblem {
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream);
 // The same for few rows; x and w fit the tensor maps.
 void gemm_few(const FfnProblem& q, int dev, cudaStream_t stream);
+double gemm_few_us(const FfnProblem& q, int dev);  // its estimated time
 // float32: sx_k and sw_k 1, or sw_n 1, or sx_m and sw_n 1; K >= 1.
 void gemm_f32(const FfnProblem& q, int dev, cudaStream_t stream);
 

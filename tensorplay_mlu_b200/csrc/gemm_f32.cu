@@ -386,15 +386,11 @@ template <int PARTS, int NT, bool W_MN, bool X_MN>
 void launch_f32(FewParams& p, const F32Operands& o, int dev, cudaStream_t stream) {
     using S = F32Shape<NT>;
     auto kern = gemm_f32_kernel<PARTS, NT, W_MN, X_MN>;
-    static bool configured[64] = {};
-    if (!configured[dev]) {
-        TPB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
-        configured[dev] = true;
-    }
+    const Slots& slots = cluster_slots<gemm_f32_kernel<PARTS, NT, W_MN, X_MN>>(S::kThreads, S::kSmem, dev);
     p.idesc = (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(NT >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     p.row_tiles = (p.M + NT - 1) / NT;
     const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
-    const int split = choose_split(tiles, p.k_blocks, num_sms(dev), 16, 16);
+    const int split = choose_split(tiles, p.k_blocks, slots, 16);
     launch_cluster(kern, tiles * split, split, S::kThreads, S::kSmem, stream, p, o);
     check_launch("gemm_f32");
 }

@@ -185,54 +185,60 @@ __global__ void __launch_bounds__(kFewThreads)
     }
 }
 
+// Launches the product, or with `us` only estimates its time.
 template <typename T, int PARTS, int NT, bool W_MN>
-void launch_few(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType type, FewParams& p, int dev,
-                cudaStream_t stream) {
+void launch_few(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
     using S = FewShape<NT>;
     auto kern = gemm_few_kernel<T, PARTS, NT, W_MN>;
-    static bool configured[64] = {};
-    if (!configured[dev]) {
-        TPB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
-        configured[dev] = true;
+    const Slots& slots = cluster_slots<gemm_few_kernel<T, PARTS, NT, W_MN>>(kFewThreads, S::kSmem, dev);
+    const int row_tiles = static_cast<int>((q.M + NT - 1) / NT), k_blocks = static_cast<int>((q.K + 63) / 64);
+    const int64_t tiles = int64_t(row_tiles) * ((q.N + 128 / PARTS - 1) / (128 / PARTS));
+    int64_t waves = 1;
+    const int split = choose_split(tiles, k_blocks, slots, 8, &waves);
+    if (us != nullptr) {
+        *us = 6.0 + waves * ((k_blocks + split - 1) / split * (tiles * split > num_sms(dev) ? 0.5 : 0.27) + 2.0);
+        return;
     }
-    const CUtensorMap mx = make_map(q.x, type, 2, q.K, q.M, q.sx_m, 1, 0, NT);
+    FewParams p = few_params(q, dev, 64);
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(W_MN) << 15) | (uint32_t(NT >> 3) << 17) |
               (uint32_t(128 >> 4) << 24);
-    p.row_tiles = (p.M + NT - 1) / NT;
-    const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
-    const int split = choose_split(tiles, p.k_blocks, int64_t(num_sms(dev)) * S::kCtas, 8, 8);
+    p.row_tiles = row_tiles;
+    const CUtensorMap mx = make_map(q.x, type, 2, q.K, q.M, q.sx_m, 1, 0, NT);
+    const CUtensorMap mw = W_MN ? make_map(q.w, type, 2, q.N, q.K, q.sw_k, 1, 0, 64)
+                                : make_map(q.w, type, 2, q.K, PARTS * q.N, q.sw_n, 1, 0, kBoxRows);
     launch_cluster(kern, tiles * split, split, kFewThreads, S::kSmem, stream, mw, mx, p);
     check_launch("gemm_few");
 }
 
 template <typename T, int PARTS, bool W_MN>
-void launch_rows(const FfnProblem& q, const CUtensorMap& mw, CUtensorMapDataType type, FewParams& p, int dev,
-                 cudaStream_t stream) {
-    if (q.M <= 16) launch_few<T, PARTS, 16, W_MN>(q, mw, type, p, dev, stream);
-    else if (q.M <= 32) launch_few<T, PARTS, 32, W_MN>(q, mw, type, p, dev, stream);
-    else if (q.M <= 64) launch_few<T, PARTS, 64, W_MN>(q, mw, type, p, dev, stream);
-    else launch_few<T, PARTS, 128, W_MN>(q, mw, type, p, dev, stream);
+void launch_rows(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
+    if (q.M <= 16) launch_few<T, PARTS, 16, W_MN>(q, type, dev, stream, us);
+    else if (q.M <= 32) launch_few<T, PARTS, 32, W_MN>(q, type, dev, stream, us);
+    else if (q.M <= 64) launch_few<T, PARTS, 64, W_MN>(q, type, dev, stream, us);
+    else launch_few<T, PARTS, 128, W_MN>(q, type, dev, stream, us);
 }
 
 template <typename T>
-void launch_typed(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream) {
-    FewParams p = few_params(q, dev, 64);
-    if (q.sw_k != 1) {
-        const CUtensorMap mw = make_map(q.w, type, 2, q.N, q.K, q.sw_k, 1, 0, 64);
-        launch_rows<T, 1, true>(q, mw, type, p, dev, stream);
-    } else {
-        const CUtensorMap mw = make_map(q.w, type, 2, q.K, q.parts * q.N, q.sw_n, 1, 0, kBoxRows);
-        if (q.parts == 2) launch_rows<T, 2, false>(q, mw, type, p, dev, stream);
-        else launch_rows<T, 1, false>(q, mw, type, p, dev, stream);
-    }
+void launch_typed(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
+    if (q.sw_k != 1) launch_rows<T, 1, true>(q, type, dev, stream, us);
+    else if (q.parts == 2) launch_rows<T, 2, false>(q, type, dev, stream, us);
+    else launch_rows<T, 1, false>(q, type, dev, stream, us);
+}
+
+void dispatch(const FfnProblem& q, int dev, cudaStream_t stream, double* us) {
+    if (q.dtype == TPB_BF16) launch_typed<__nv_bfloat16>(q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dev, stream, us);
+    else launch_typed<__half>(q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dev, stream, us);
 }
 
 }  // namespace
 
-void gemm_few(const FfnProblem& q, int dev, cudaStream_t stream) {
-    if (q.dtype == TPB_BF16) launch_typed<__nv_bfloat16>(q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dev, stream);
-    else launch_typed<__half>(q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dev, stream);
+void gemm_few(const FfnProblem& q, int dev, cudaStream_t stream) { dispatch(q, dev, stream, nullptr); }
+
+double gemm_few_us(const FfnProblem& q, int dev) {
+    double us = 0.0;
+    dispatch(q, dev, nullptr, &us);
+    return us;
 }
 
 }  // namespace tpb

@@ -23,18 +23,6 @@
 namespace tpb {
 namespace {
 
-// The residual's rows, where 16-byte loads cannot read them, into a staging
-// tile.
-template <typename T>
-__device__ __forceinline__ void load_staged_rows(uint8_t* stage, int lane, const T* src, int64_t pitch, int64_t cols,
-                                                 int64_t rows) {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-        const T v = r < rows && lane < cols ? src[r * pitch + lane] : T(0.0f);
-        *reinterpret_cast<T*>(stage + stage_offset(2, r, lane)) = v;
-    }
-}
-
 // bias[n .. n + 32) added to a chunk (every lane reads the same addresses).
 template <typename T>
 __device__ __forceinline__ void add_bias_chunk(const T* bias, int64_t n, int64_t N, float (&z)[32]) {
@@ -95,14 +83,23 @@ __device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUten
 #pragma unroll
         for (int q = 0; q < kParts; ++q) tmem_ld32(t_rows + c0 + q * 128, raw[q]);
         // The residual's loads are in flight while the accumulator arrives.
-        Vec<T, 8> res[4];
-        bool res_vec = false;
-        if (f.residual != nullptr && lane < rows) {
-            const T* r = static_cast<const T*>(f.residual) + (row0 + lane) * f.sres_m + n;
-            res_vec = f.residual_vec && cols >= 32;
+        // Rows on 16-byte boundaries: a lane's own row.  Others: a lane's own
+        // column, transposed through the staging tile below.
+        Vec<T, 32> res;
+        const bool res_vec = f.residual_vec && cols >= 32;
+        if (EPI == kEpiAct && f.residual != nullptr) {
+            const T* r = static_cast<const T*>(f.residual) + row0 * f.sres_m + n;
             if (res_vec) {
+                if (lane < rows) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) res[q] = reinterpret_cast<const Vec<T, 8>*>(r)[q];
+                    for (int q = 0; q < 4; ++q) {
+                        reinterpret_cast<Vec<T, 8>*>(&res)[q] =
+                            reinterpret_cast<const Vec<T, 8>*>(r + lane * f.sres_m)[q];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) res.v[i] = i < rows && lane < cols ? r[i * f.sres_m + lane] : T(0.0f);
             }
         }
         tmem_wait_ld();
@@ -169,26 +166,23 @@ __device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUten
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[0][j] *= z[1][j];
         }
-        if (f.residual != nullptr) {
-            if (f.residual_vec && cols >= 32) {
-                if (res_vec) {
+        if (EPI == kEpiAct && f.residual != nullptr) {
+            if (!res_vec) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float r[8];
-                        unpack_vec(res[q], r);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) z[0][q * 8 + j] += r[j];
-                    }
-                }
-            } else {
-                load_staged_rows<T>(stage, lane, static_cast<const T*>(f.residual) + row0 * f.sres_m + n, f.sres_m, cols,
-                                    rows);
+                for (int i = 0; i < 32; ++i) *reinterpret_cast<T*>(stage + stage_offset(2, i, lane)) = res.v[i];
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    z[0][j] += load_as<float>(*reinterpret_cast<const T*>(stage + stage_offset(2, lane, j)));
+                for (int q = 0; q < 4; ++q) {
+                    reinterpret_cast<Vec<T, 8>*>(&res)[q] =
+                        *reinterpret_cast<const Vec<T, 8>*>(stage + stage_offset(2, lane, q * 8));
                 }
                 __syncwarp();
+            }
+            if (lane < rows) {
+                float r[32];
+                unpack_vec(res, r);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) z[0][j] += r[j];
             }
         }
         Vec<T, 32> packed;
@@ -275,10 +269,20 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
 
 }  // namespace
 
-// Whether the few-row kernel takes a product.
-bool few_rows(const FfnProblem& q, int) {
-    static const int limit = std::getenv("TPB200_FFN_FEW") ? std::atoi(std::getenv("TPB200_FFN_FEW")) : 128;
-    return q.M <= limit;
+// Whether the split-K kernel (gemm_few.cu) takes a product: up to 64 rows
+// always (its bound is the weight's one reading), beyond where its estimated
+// time is below this kernel's.  Measured, bf16, us, pair / split: 100 rows x
+// 4096 -> 512: 27 / 9; 384 x 4096 -> 2048: 28 / 23; 576 x 1024 -> 2048: 12.6 /
+// 11.3; 1024 x 1024 -> 2048: 12.7 / 13.6; 2048 x 4096 -> 6000: 79 / 108.  The
+// estimate here: 0.31 us for each 64-deep step of a wave of 256 x 256 tiles,
+// 2.2 us for a wave's ramp and epilogue, 5 us once.
+bool few_rows(const FfnProblem& q, int dev) {
+    if (q.M <= 64) return true;
+    const int64_t columns = q.parts == 2 ? 128 : kPairBN;
+    const int64_t tiles = ((q.M + kPairBM - 1) / kPairBM) * ((q.N + columns - 1) / columns);
+    const int64_t clusters = std::max(1, gemm_sm_budget(dev) / 2);
+    const double waves = static_cast<double>((tiles + clusters - 1) / clusters);
+    return gemm_few_us(q, dev) < 5.0 + waves * (0.3125 * static_cast<double>((q.K + 63) / 64) + 2.2);
 }
 
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {

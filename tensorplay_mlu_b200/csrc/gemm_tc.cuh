@@ -358,15 +358,38 @@ __device__ __forceinline__ int stage_offset(int es, int r, int c) {
 }
 
 // A staged 32 x 32 tile to rows that TMA cannot store (off 16-byte
-// boundaries): a row at a time, one element a lane.
+// boundaries), in units of U bytes that all rows start on a boundary of: one
+// instruction stores 32 U / (32 sizeof(T)) rows.
+template <typename T, typename U>
+__device__ __forceinline__ void store_staged_units(const uint8_t* stage, int lane, T* dst, int64_t pitch, int64_t cols,
+                                                   int64_t rows) {
+    constexpr int kPer = sizeof(U) / sizeof(T);       // elements of a unit
+    constexpr int kLanes = 32 / kPer;                 // lanes of a row
+    const int c = (lane % kLanes) * kPer;
+#pragma unroll 8
+    for (int r = lane / kLanes; r < 32; r += kPer) {
+        if (r >= rows) break;
+        const uint8_t* at = stage + stage_offset(sizeof(T), r, c);
+        if (c + kPer <= cols) {
+            *reinterpret_cast<U*>(dst + r * pitch + c) = *reinterpret_cast<const U*>(at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                if (c + e < cols) dst[r * pitch + c + e] = reinterpret_cast<const T*>(at)[e];
+            }
+        }
+    }
+}
 template <typename T>
 __device__ __forceinline__ void store_staged_rows(const uint8_t* stage, int lane, T* dst, int64_t pitch, int64_t cols,
                                                   int64_t rows) {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-        if (r < rows && lane < cols) {
-            dst[r * pitch + lane] = *reinterpret_cast<const T*>(stage + stage_offset(sizeof(T), r, lane));
-        }
+    const uint32_t low = uint32_t(reinterpret_cast<uintptr_t>(dst)) | uint32_t(pitch * int64_t(sizeof(T)));
+    if (low % 8 == 0) store_staged_units<T, uint64_t>(stage, lane, dst, pitch, cols, rows);
+    else if constexpr (sizeof(T) < 4) {
+        if (low % 4 == 0) store_staged_units<T, uint32_t>(stage, lane, dst, pitch, cols, rows);
+        else store_staged_units<T, T>(stage, lane, dst, pitch, cols, rows);
+    } else {
+        store_staged_units<T, T>(stage, lane, dst, pitch, cols, rows);
     }
 }
 
