@@ -8,9 +8,9 @@
 //   * the weight is the MMA's 128-row operand and the rows of x its N
 //     dimension (kNT = 16 .. 128), so no tensor work goes into padding rows
 //     beyond the next 16;
-//   * a gated tile is 64 gate rows and 64 up rows of the weight, so both
-//     operators stage the same 128 rows and two CTAs fit an SM: one's set-up
-//     and final sum overlap the other's stream;
+//   * a gated tile is 64 gate rows and 64 up rows of the weight, or 128 and
+//     128 for up to 32 rows of x; two CTAs fit an SM, and one's set-up and
+//     final sum overlap the other's stream;
 //   * K is split over a cluster of C CTAs, because N / 128 tiles alone do not
 //     fill 148 SMs; each CTA streams its share of K through a TMA ring into
 //     TMEM accumulators;
@@ -24,6 +24,8 @@
 // Every wait is bounded as in gemm_tc.cu; all threads reach the cluster
 // barriers.  No TMA multicast is used.
 
+#include <cmath>
+
 #include "gemm_few.cuh"
 
 namespace tpb {
@@ -32,25 +34,26 @@ namespace {
 constexpr int kFewThreads = 192;  // warp 0 TMA producer, 1 MMA issuer, 2-5 accumulator readers
 constexpr int kFewWarps = kFewThreads / 32;
 
-template <int NT>
+// WT: 128-row accumulators of a tile.
+template <int NT, int WT>
 struct FewShape {
-    static constexpr uint32_t kWBytes = 128 * 128;
+    static constexpr uint32_t kWBytes = WT * 128 * 128;
     static constexpr uint32_t kXBytes = NT * 128;
     static constexpr uint32_t kStageBytes = kWBytes + kXBytes;
-    static constexpr int kCtas = 2;  // per SM, 110 KB of stages each
+    // Two CTAs an SM, 110 KB of stages each.
     static constexpr int kStages = int(110 * 1024 / kStageBytes);
-    static constexpr uint32_t kPartialBytes = NT * 128 * 4;  // reuses the stages
+    static constexpr uint32_t kPartialBytes = WT * NT * 128 * 4;  // reuses the stages
     static_assert(kPartialBytes <= kStages * kStageBytes, "partial sums fit the stages");
     static constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024 + 256;
-    static constexpr int kTmemCols = NT < 32 ? 32 : NT;  // a power of two
+    static constexpr int kTmemCols = WT * NT < 32 ? 32 : WT * NT;  // a power of two
 };
 
-template <typename T, int PARTS, int NT, bool W_MN>
+template <typename T, int PARTS, int NT, int WT, bool W_MN>
 __global__ void __launch_bounds__(kFewThreads)
     gemm_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const FewParams p) {
-    using S = FewShape<NT>;
+    using S = FewShape<NT, WT>;
     constexpr int kStages = S::kStages;
-    constexpr int kColumns = 128 / PARTS;  // result columns of a tile
+    constexpr int kColumns = WT * 128 / PARTS;  // result columns of a tile
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * S::kStageBytes);
@@ -138,9 +141,12 @@ __global__ void __launch_bounds__(kFewThreads)
                 const uint32_t at = smem_addr(smem + stage * S::kStageBytes);
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t ad = sw128_desc(at + kk * a_kstep, a_lbo, 1024);
                     const uint64_t bd = sw128_desc(at + S::kWBytes + kk * 32, 16, 1024);
-                    umma<false>(tmem, ad, bd, p.idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+#pragma unroll
+                    for (int t = 0; t < WT; ++t) {
+                        const uint64_t ad = sw128_desc(at + t * 16384 + kk * a_kstep, a_lbo, 1024);
+                        umma<false>(tmem + t * NT, ad, bd, p.idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
+                    }
                 }
                 umma_commit(smem_addr(&empty[stage]));
                 if (++stage == kStages) {
@@ -162,8 +168,8 @@ __global__ void __launch_bounds__(kFewThreads)
             tc_fence_after();
             float* partial = reinterpret_cast<float*>(smem);
 #pragma unroll
-            for (int c = 0; c < NT; c += 16) {
-                if (c >= p.M - m0) break;  // rows of x past M
+            for (int c = 0; c < WT * NT; c += 16) {
+                if (c % NT >= p.M - m0) continue;  // rows of x past M
                 uint32_t r[16];
                 tmem_ld16(tmem + (uint32_t(quad * 32) << 16) + c, r);
                 tmem_wait_ld();
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(kFewThreads)
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // every CTA's partial sums are in its shared memory
-    finish_rows<T, PARTS, NT>(p, reinterpret_cast<const float*>(smem), m0, n0, warp, kFewWarps, rank, ranks,
+    finish_rows<T, PARTS, NT, (WT > 1)>(p, reinterpret_cast<const float*>(smem), m0, n0, warp, kFewWarps, rank, ranks,
                               [](int64_t, int64_t, int, float&) {});
     cluster_sync();  // no CTA leaves while another reads its shared memory
     if (warp == 1) {
@@ -185,16 +191,48 @@ __global__ void __launch_bounds__(kFewThreads)
     }
 }
 
+// Microseconds of a product of few rows, which streams its weight: n CTAs of
+// `mb` megabytes each, at most `slots` at a time.  What n CTAs draw together
+// saturates: 3.5 TB/s was measured for 64 of them, 5.7 for 172, 6.2 for 256,
+// close to 6.5 (1 - exp(-n / 92)); a wave's ramp takes 2.5 us, the cluster's
+// sum 0.1 us a rank.  (4096 -> 2 * 11008, one token: 64 + 64 columns 35.5 /
+// measured 34 - 38 us, 128 + 128 with K split by three 32.5 / 30.7 us; 2 *
+// 16384: 46.5 / 45.0, 46.6 / 47.0.)
+double stream_us(int64_t n, int64_t slots, double mb, int split) {
+    const auto wave = [&](int64_t ctas) { return ctas * mb / (6.5 * (1.0 - std::exp(-double(ctas) / 92.0))) + 2.5; };
+    const int64_t full = n / slots, rest = n - full * slots;
+    return (full > 0 ? full * wave(slots) : 0.0) + (rest > 0 ? wave(rest) : 0.0) + 0.1 * split;
+}
+
 // Launches the product, or with `us` only estimates its time.
-template <typename T, int PARTS, int NT, bool W_MN>
+template <typename T, int PARTS, int NT, int WT, bool W_MN>
 void launch_few(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
-    using S = FewShape<NT>;
-    auto kern = gemm_few_kernel<T, PARTS, NT, W_MN>;
-    const Slots& slots = cluster_slots<gemm_few_kernel<T, PARTS, NT, W_MN>>(kFewThreads, S::kSmem, dev);
+    using S = FewShape<NT, WT>;
+    auto kern = gemm_few_kernel<T, PARTS, NT, WT, W_MN>;
+    const Slots& slots = cluster_slots<gemm_few_kernel<T, PARTS, NT, WT, W_MN>>(kFewThreads, S::kSmem, dev);
     const int row_tiles = static_cast<int>((q.M + NT - 1) / NT), k_blocks = static_cast<int>((q.K + 63) / 64);
-    const int64_t tiles = int64_t(row_tiles) * ((q.N + 128 / PARTS - 1) / (128 / PARTS));
+    const int64_t tiles = int64_t(row_tiles) * ((q.N + WT * 128 / PARTS - 1) / (WT * 128 / PARTS));
     int64_t waves = 1;
-    const int split = choose_split(tiles, k_blocks, slots, 8, &waves);
+    int split = 1;
+    double stream_best = 1e30;
+    if constexpr (NT <= 64) {
+        // A block's weight rows, and its rows of x from L2 at a fraction of
+        // their cost.
+        const double block_mb = (S::kWBytes + 0.4 * S::kXBytes) * 1e-6;
+        for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
+            const double t = stream_us(tiles * c, slots.ctas[c], block_mb * ((k_blocks + c - 1) / c), c);
+            if (t < stream_best) {
+                stream_best = t;
+                split = c;
+            }
+        }
+        if (us != nullptr) {
+            *us = stream_best;
+            return;
+        }
+    } else {
+        split = choose_split(tiles, k_blocks, slots, 8, &waves);
+    }
     if (us != nullptr) {
         *us = 6.0 + waves * ((k_blocks + split - 1) / split * (tiles * split > num_sms(dev) ? 0.5 : 0.27) + 2.0);
         return;
@@ -211,12 +249,28 @@ void launch_few(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStre
     check_launch("gemm_few");
 }
 
+// Gated tiles of 64 + 64 or 128 + 128 columns, whichever fills the device
+// better.
+template <typename T, int PARTS, int NT, bool W_MN>
+void launch_narrow(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
+    if constexpr (PARTS == 2) {
+        double one = 0.0, two = 0.0;
+        launch_few<T, PARTS, NT, 1, W_MN>(q, type, dev, stream, &one);
+        launch_few<T, PARTS, NT, 2, W_MN>(q, type, dev, stream, &two);
+        if (us != nullptr) *us = std::min(one, two);
+        else if (two < one) launch_few<T, PARTS, NT, 2, W_MN>(q, type, dev, stream, nullptr);
+        else launch_few<T, PARTS, NT, 1, W_MN>(q, type, dev, stream, nullptr);
+    } else {
+        launch_few<T, PARTS, NT, 1, W_MN>(q, type, dev, stream, us);
+    }
+}
+
 template <typename T, int PARTS, bool W_MN>
 void launch_rows(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
-    if (q.M <= 16) launch_few<T, PARTS, 16, W_MN>(q, type, dev, stream, us);
-    else if (q.M <= 32) launch_few<T, PARTS, 32, W_MN>(q, type, dev, stream, us);
-    else if (q.M <= 64) launch_few<T, PARTS, 64, W_MN>(q, type, dev, stream, us);
-    else launch_few<T, PARTS, 128, W_MN>(q, type, dev, stream, us);
+    if (q.M <= 16) launch_narrow<T, PARTS, 16, W_MN>(q, type, dev, stream, us);
+    else if (q.M <= 32) launch_narrow<T, PARTS, 32, W_MN>(q, type, dev, stream, us);
+    else if (q.M <= 64) launch_few<T, PARTS, 64, 1, W_MN>(q, type, dev, stream, us);
+    else launch_few<T, PARTS, 128, 1, W_MN>(q, type, dev, stream, us);
 }
 
 template <typename T>

@@ -135,15 +135,18 @@ __device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_
 
 // Sums a tile over the cluster's ranks and finishes it.  partial: a CTA's sums,
 // [row of x][row of the weight tile] floats at the same address in every
-// rank.  Warp `warp` of `warps` takes every warps-th row of x of this rank's
+// rank; with kWide, a gated tile of 128 columns, [part][row of x][column].  Warp `warp` of `warps` takes every warps-th row of x of this rank's
 // share, each lane V columns of it, four ranks' loads in flight at a time,
 // added in rank order.  fix(row of x, result column, part, z): a chance to
 // replace a sum.
-template <typename T, int PARTS, int NT, typename Fix>
+template <typename T, int PARTS, int NT, bool kWide = false, typename Fix>
 __device__ __forceinline__ void finish_rows(const FewParams& p, const float* partial, int m0, int n0, int warp,
                                             int warps, int rank, int ranks, Fix fix) {
-    constexpr int kColumns = 128 / PARTS;  // result columns of a tile
+    constexpr int kColumns = kWide ? 128 : 128 / PARTS;  // result columns of a tile
     constexpr int kV = kColumns / 32;
+    const auto offset = [](int m, int q, int lane) {
+        return (kWide ? (q * NT + m) * 128 : m * 128 + q * kColumns) + lane * kV;
+    };
     const int lane = threadIdx.x & 31;
     const int rows = min(NT, p.M - m0);
     const int64_t n = int64_t(n0) + lane * kV;
@@ -154,7 +157,7 @@ __device__ __forceinline__ void finish_rows(const FewParams& p, const float* par
             float z[PARTS][kV];
 #pragma unroll
             for (int q = 0; q < PARTS; ++q) {
-                const Vec<float, kV> v = *reinterpret_cast<const Vec<float, kV>*>(partial + m * 128 + q * kColumns + lane * kV);
+                const Vec<float, kV> v = *reinterpret_cast<const Vec<float, kV>*>(partial + offset(m, q, lane));
 #pragma unroll
                 for (int j = 0; j < kV; ++j) {
                     z[q][j] = v.v[j];
@@ -169,7 +172,7 @@ __device__ __forceinline__ void finish_rows(const FewParams& p, const float* par
         float z[PARTS][kV];
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
-            const uint32_t at = smem_addr(partial) + uint32_t(m * 128 + q * kColumns + lane * kV) * 4;
+            const uint32_t at = smem_addr(partial + offset(m, q, lane));
 #pragma unroll
             for (int j = 0; j < kV; ++j) z[q][j] = 0.0f;
             for (int c0 = 0; c0 < ranks; c0 += 4) {
