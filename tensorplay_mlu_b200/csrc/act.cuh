@@ -18,49 +18,40 @@
 namespace tpb {
 namespace {
 
-template <bool Fast>
-__device__ __forceinline__ float sigmoid_of(float z) {
-    if constexpr (Fast) return rcp_approx(1.0f + __expf(-z));
-    else return 1.0f / (1.0f + expf(-z));
-}
-
-template <bool Fast>
-__device__ __forceinline__ float phi_of(float z) {
-    if constexpr (Fast) return phi_narrow(z);
-    else return normcdff(z);
-}
-
 constexpr float kTanhBeta = 0.79788456080286535588f;  // sqrt(2 / pi)
 constexpr float kTanhKappa = 0.044715f;
 
-template <int ACT, bool Fast>
+// ---- fp32 results: accurate functions, one element at a time --------------
+
+__device__ __forceinline__ float sigmoid_of(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
     if constexpr (ACT == TPB_ACT_RELU) return (z > 0.0f || z != z) ? z : 0.0f;
-    else if constexpr (ACT == TPB_ACT_GELU) return z * phi_of<Fast>(z);
+    else if constexpr (ACT == TPB_ACT_GELU) return z * normcdff(z);
     else if constexpr (ACT == TPB_ACT_GELU_TANH) {
-        return z * sigmoid_of<Fast>(2.0f * kTanhBeta * fmaf(kTanhKappa * z * z, z, z));
-    } else if constexpr (ACT == TPB_ACT_SILU) return z * sigmoid_of<Fast>(z);
+        return z * sigmoid_of(2.0f * kTanhBeta * fmaf(kTanhKappa * z * z, z, z));
+    } else if constexpr (ACT == TPB_ACT_SILU) return z * sigmoid_of(z);
     else return z;
 }
 
 // The activation and its slope from one evaluation of the gate.
-template <int ACT, bool Fast>
+template <int ACT>
 __device__ __forceinline__ void act_slope(float z, float& a, float& d) {
     if constexpr (ACT == TPB_ACT_RELU) {
         a = (z > 0.0f || z != z) ? z : 0.0f;
         d = z <= 0.0f ? 0.0f : 1.0f;
     } else if constexpr (ACT == TPB_ACT_GELU) {
-        const float g = phi_of<Fast>(z);
-        const float e = Fast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
+        const float g = normcdff(z);
         a = z * g;
-        d = fmaf(z * 0.39894228040143267794f, e, g);  // phi(z) = exp(-z^2 / 2) / sqrt(2 pi)
+        d = fmaf(z * 0.39894228040143267794f, expf(-0.5f * z * z), g);  // phi(z) = exp(-z^2 / 2) / sqrt(2 pi)
     } else if constexpr (ACT == TPB_ACT_GELU_TANH) {
         const float z2 = z * z;
-        const float g = sigmoid_of<Fast>(2.0f * kTanhBeta * fmaf(kTanhKappa * z2, z, z));
+        const float g = sigmoid_of(2.0f * kTanhBeta * fmaf(kTanhKappa * z2, z, z));
         a = z * g;
         d = fmaf(a * (1.0f - g), 2.0f * kTanhBeta * fmaf(3.0f * kTanhKappa, z2, 1.0f), g);
     } else if constexpr (ACT == TPB_ACT_SILU) {
-        const float g = sigmoid_of<Fast>(z);
+        const float g = sigmoid_of(z);
         a = z * g;
         d = fmaf(a, 1.0f - g, g);
     } else {
@@ -69,20 +60,115 @@ __device__ __forceinline__ void act_slope(float z, float& a, float& d) {
     }
 }
 
-// z[j] <- act(z[j]); the switch is uniform over the grid and sits outside the
-// unrolled loop.
+// ---- 16-bit results: two lanes at a time ------------------------------------
+//
+// The packed two-lane instructions halve the arithmetic, which otherwise costs
+// more than the memory traffic of these passes (gelu's slope: 222 us over
+// 8192 x 16384 bf16 from 8 bits, against 103 us for the bytes).
+
+// 1 / (1 + 2^t): exp2 overflowing to infinity gives 0.
+__device__ __forceinline__ float2 gate_of_exp2(float2 t) {
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = __fadd2_rn(e, f2(1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    return r;
+}
+
+constexpr float kLog2E = 1.44269504088896340736f;
+
+template <int ACT>
+__device__ __forceinline__ float2 gate2(float2 z, float2 z2) {
+    if constexpr (ACT == TPB_ACT_GELU) {
+        return phi_narrow2(z);
+    } else if constexpr (ACT == TPB_ACT_GELU_TANH) {
+        // sigmoid(2 u) = 1 / (1 + 2^(-2 log2(e) u)), u = beta (z + kappa z^3)
+        const float2 c = __ffma2_rn(z2, f2(-2.0f * kLog2E * kTanhBeta * kTanhKappa), f2(-2.0f * kLog2E * kTanhBeta));
+        return gate_of_exp2(__fmul2_rn(z, c));
+    } else {
+        return gate_of_exp2(__fmul2_rn(z, f2(-kLog2E)));
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 act_value2(float2 z) {
+    if constexpr (ACT == TPB_ACT_NONE || ACT == TPB_ACT_RELU) {
+        return make_float2(act_value<ACT>(z.x), act_value<ACT>(z.y));
+    } else {
+        return __fmul2_rn(z, gate2<ACT>(z, __fmul2_rn(z, z)));
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_slope2(float2 z, float2& a, float2& d) {
+    if constexpr (ACT == TPB_ACT_NONE || ACT == TPB_ACT_RELU) {
+        act_slope<ACT>(z.x, a.x, d.x);
+        act_slope<ACT>(z.y, a.y, d.y);
+    } else {
+        const float2 z2 = __fmul2_rn(z, z);
+        const float2 g = gate2<ACT>(z, z2);
+        a = __fmul2_rn(z, g);
+        if constexpr (ACT == TPB_ACT_GELU) {
+            const float2 t = __fmul2_rn(z2, f2(-0.5f * kLog2E));
+            float2 e;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+            d = __ffma2_rn(__fmul2_rn(z, f2(0.39894228040143267794f)), e, g);
+        } else {
+            const float2 h = __ffma2_rn(g, f2(-1.0f), f2(1.0f));  // 1 - g
+            float2 slope = __fmul2_rn(a, h);
+            if constexpr (ACT == TPB_ACT_GELU_TANH) {
+                slope = __fmul2_rn(slope, __ffma2_rn(z2, f2(6.0f * kTanhBeta * kTanhKappa), f2(2.0f * kTanhBeta)));
+            }
+            d = __fadd2_rn(slope, g);
+        }
+    }
+}
+
+// z[j] <- act(z[j]), and act and its slope; the switch is uniform over the
+// grid and sits outside the unrolled loops.
+template <int ACT, bool Fast, int V>
+__device__ __forceinline__ void act_values_of(float (&z)[V]) {
+    if constexpr (Fast && V % 2 == 0) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            const float2 r = act_value2<ACT>(make_float2(z[j], z[j + 1]));
+            z[j] = r.x;
+            z[j + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = act_value<ACT>(z[j]);
+    }
+}
+
+template <int ACT, bool Fast, int V>
+__device__ __forceinline__ void act_slopes_of(const float (&z)[V], float (&a)[V], float (&d)[V]) {
+    if constexpr (Fast && V % 2 == 0) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            float2 va, vd;
+            act_slope2<ACT>(make_float2(z[j], z[j + 1]), va, vd);
+            a[j] = va.x;
+            a[j + 1] = va.y;
+            d[j] = vd.x;
+            d[j + 1] = vd.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) act_slope<ACT>(z[j], a[j], d[j]);
+    }
+}
+
 template <bool Fast, int V>
 __device__ __forceinline__ void act_values(int act, float (&z)[V]) {
     switch (act) {
-#define TPB_ACT_CASE(A)                                            \
-    case A:                                                        \
-        _Pragma("unroll") for (int j = 0; j < V; ++j) z[j] = act_value<A, Fast>(z[j]); \
-        break;
-        TPB_ACT_CASE(TPB_ACT_RELU)
-        TPB_ACT_CASE(TPB_ACT_GELU)
-        TPB_ACT_CASE(TPB_ACT_GELU_TANH)
-        TPB_ACT_CASE(TPB_ACT_SILU)
-#undef TPB_ACT_CASE
+        case TPB_ACT_RELU: act_values_of<TPB_ACT_RELU, Fast, V>(z); break;
+        case TPB_ACT_GELU: act_values_of<TPB_ACT_GELU, Fast, V>(z); break;
+        case TPB_ACT_GELU_TANH: act_values_of<TPB_ACT_GELU_TANH, Fast, V>(z); break;
+        case TPB_ACT_SILU: act_values_of<TPB_ACT_SILU, Fast, V>(z); break;
         default: break;
     }
 }
@@ -90,19 +176,11 @@ __device__ __forceinline__ void act_values(int act, float (&z)[V]) {
 template <bool Fast, int V>
 __device__ __forceinline__ void act_slopes(int act, const float (&z)[V], float (&a)[V], float (&d)[V]) {
     switch (act) {
-#define TPB_ACT_CASE(A)                                            \
-    case A:                                                        \
-        _Pragma("unroll") for (int j = 0; j < V; ++j) act_slope<A, Fast>(z[j], a[j], d[j]); \
-        break;
-        TPB_ACT_CASE(TPB_ACT_RELU)
-        TPB_ACT_CASE(TPB_ACT_GELU)
-        TPB_ACT_CASE(TPB_ACT_GELU_TANH)
-        TPB_ACT_CASE(TPB_ACT_SILU)
-#undef TPB_ACT_CASE
-        default: {
-#pragma unroll
-            for (int j = 0; j < V; ++j) act_slope<TPB_ACT_NONE, Fast>(z[j], a[j], d[j]);
-        }
+        case TPB_ACT_RELU: act_slopes_of<TPB_ACT_RELU, Fast, V>(z, a, d); break;
+        case TPB_ACT_GELU: act_slopes_of<TPB_ACT_GELU, Fast, V>(z, a, d); break;
+        case TPB_ACT_GELU_TANH: act_slopes_of<TPB_ACT_GELU_TANH, Fast, V>(z, a, d); break;
+        case TPB_ACT_SILU: act_slopes_of<TPB_ACT_SILU, Fast, V>(z, a, d); break;
+        default: act_slopes_of<TPB_ACT_NONE, Fast, V>(z, a, d);
     }
 }
 
@@ -144,8 +222,56 @@ __device__ __forceinline__ float ckpt_inverse(int stored) { return __uint_as_flo
 __device__ __forceinline__ float ckpt_step(int stored) {
     return stored == kCkptNonFinite ? __int_as_float(0x7fffffff) : __uint_as_float(uint32_t(stored) << 23);
 }
-__device__ __forceinline__ int8_t ckpt_quantise(float x, float inverse, float qmax) {
-    return static_cast<int8_t>(__float2int_rn(fminf(fmaxf(x * inverse, -qmax), qmax)));
+
+// V values (1, 2, or a multiple of 4) of a block as int8.  Adding 1.5 * 2^23
+// rounds to the nearest integer, ties to even, and leaves it in the low byte
+// of the sum's bits: a full-rate addition instead of a conversion.  stored:
+// the block's exponent; qmax below 127 clamps (see ckpt_exponent).
+template <int V>
+__device__ __forceinline__ Vec<int8_t, V> ckpt_quantise(const float (&x)[V], int stored, float qmax) {
+    const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+    uint32_t bits[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float q = x[j] * inverse;
+        if (qmax < 127.0f) q = fminf(fmaxf(q, -qmax), qmax);  // one block in a type's last binade; NaN * 0 = 0
+        bits[j] = __float_as_uint(q + 12582912.0f);
+    }
+    Vec<int8_t, V> out;
+    if constexpr (V % 4 == 0) {
+        uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            o[j / 4] = __byte_perm(__byte_perm(bits[j], bits[j + 1], 0x0040), __byte_perm(bits[j + 2], bits[j + 3], 0x0040),
+                                   0x5410);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) out.v[j] = static_cast<int8_t>(bits[j] & 0xffu);
+    }
+    return out;
+}
+
+// The values a checkpoint's bytes stand for.  A byte b with its sign bit
+// flipped is b + 128; under the exponent of 2^23 it reads 2^23 + 128 + b, from
+// which the offset is subtracted exactly: no conversion instruction.
+template <int V>
+__device__ __forceinline__ void ckpt_values(const Vec<int8_t, V>& q, int stored, float (&x)[V]) {
+    const float step = ckpt_step(stored);
+    if constexpr (V % 4 == 0) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&q);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const uint32_t u = w[j / 4] ^ 0x80808080u;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                x[j + b] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + b)) - 8388736.0f) * step;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = float(q.v[j]) * step;
+    }
 }
 
 }  // namespace

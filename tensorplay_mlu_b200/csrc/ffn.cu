@@ -13,15 +13,65 @@
 namespace tpb {
 namespace {
 
-// V consecutive elements of a row as floats: 16-byte loads for V = 8 (one for
-// 16-bit types, two for fp32), one element for V = 1.
-template <typename T, int V>
-struct RowVec {
-    static constexpr int kPer = V == 1 ? 1 : (16 / int(sizeof(T)) < V ? 16 / int(sizeof(T)) : V);
-    Vec<T, kPer> part[V / kPer];
-    __device__ __forceinline__ void load(const T* p) {
+// How a kernel's rows lie: kAligned, every chunk of V elements on a 16-byte
+// boundary (8 bytes for checkpoint values) and whole; or kAnywhere, in which
+// case chunks are read and written in the largest words they start on, and
+// a row's last one may be short.
+constexpr bool kAligned = true;
+constexpr bool kAnywhere = false;
+
+// N bytes at p in words of W bytes (p a multiple of W).
+template <typename W, int N>
+__device__ __forceinline__ void copy_in(void* to, const void* p) {
 #pragma unroll
-        for (int i = 0; i < V / kPer; ++i) part[i] = reinterpret_cast<const Vec<T, kPer>*>(p)[i];
+    for (int i = 0; i < N / int(sizeof(W)); ++i) reinterpret_cast<W*>(to)[i] = reinterpret_cast<const W*>(p)[i];
+}
+
+// V consecutive elements of E at p (`count` of them exist).
+template <typename E, int V, bool ALIGNED>
+struct Chunk {
+    static constexpr int kBytes = V * int(sizeof(E));
+    static constexpr int kPer = (16 < kBytes ? 16 : kBytes) / int(sizeof(E));
+    Vec<E, kPer> part[V / kPer];
+
+    __device__ __forceinline__ void load(const E* p, int count) {
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int i = 0; i < V / kPer; ++i) part[i] = reinterpret_cast<const Vec<E, kPer>*>(p)[i];
+        } else {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+            if (count == V && at % 4 == 0) {
+                copy_in<uint32_t, kBytes>(part, p);
+            } else if (count == V && sizeof(E) == 1 && at % 2 == 0) {
+                copy_in<uint16_t, kBytes>(part, p);
+            } else {
+                E* e = reinterpret_cast<E*>(part);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (j < count) e[j] = p[j];
+                    else memset(&e[j], 0, sizeof(E));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(E* p, int count) const {
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int i = 0; i < V / kPer; ++i) reinterpret_cast<Vec<E, kPer>*>(p)[i] = part[i];
+        } else {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+            if (count == V && at % 4 == 0) {
+                copy_in<uint32_t, kBytes>(p, part);
+            } else if (count == V && sizeof(E) == 1 && at % 2 == 0) {
+                copy_in<uint16_t, kBytes>(p, part);
+            } else {
+                const E* e = reinterpret_cast<const E*>(part);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (j < count) p[j] = e[j];
+                }
+            }
+        }
     }
     __device__ __forceinline__ void get(float (&f)[V]) const {
 #pragma unroll
@@ -41,9 +91,14 @@ struct RowVec {
             pack_vec(t, part[i]);
         }
     }
-    __device__ __forceinline__ void store(T* p) const {
-#pragma unroll
-        for (int i = 0; i < V / kPer; ++i) reinterpret_cast<Vec<T, kPer>*>(p)[i] = part[i];
+};
+
+// A checkpoint's int8 values, V of them.
+template <int V, bool ALIGNED>
+struct ByteChunk : Chunk<int8_t, V, ALIGNED> {
+    __device__ __forceinline__ const Vec<int8_t, V>& all() const {
+        static_assert(V <= 16, "one part");
+        return this->part[0];
     }
 };
 
@@ -67,8 +122,9 @@ Units make_units(int64_t rows, int64_t n) {
     return u;
 }
 
-// One block's values and exponent, from V elements in each of its lanes.
-template <typename T, int V>
+// One block's values and exponent, from V elements in each of its lanes (zero
+// past the row's end; `count` of them exist).
+template <typename T, int V, bool ALIGNED>
 __device__ __forceinline__ void pack_block(const float (&x)[V], int count, int lane_in_block, int8_t* values,
                                            uint8_t* exponent) {
     float amax = 0.0f;
@@ -78,11 +134,11 @@ __device__ __forceinline__ void pack_block(const float (&x)[V], int count, int l
     for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     float qmax;
     const int stored = ckpt_exponent<T>(amax, qmax);
-    const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
-    Vec<int8_t, V> q;
-#pragma unroll
-    for (int j = 0; j < V; ++j) q.v[j] = ckpt_quantise(x[j], inverse, qmax);
-    if (count == V) *reinterpret_cast<Vec<int8_t, V>*>(values) = q;
+    if (count > 0) {
+        Chunk<int8_t, V, ALIGNED> q;
+        q.part[0] = ckpt_quantise<V>(x, stored, qmax);
+        q.store(values, count);
+    }
     if (lane_in_block == 0 && exponent != nullptr) *exponent = static_cast<uint8_t>(stored);
 }
 
@@ -104,40 +160,41 @@ struct ForwardParams {
 // y = act(z0) [* z1] [+ residual] and the checkpoint of z0 [and z1]; a thread
 // holds V elements of a unit, kU units at a time so that their loads are in
 // flight together.
-template <typename T, int V, bool GATED>
+template <typename T, int V, bool GATED, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) ffn_forward_kernel(const ForwardParams<T> p) {
     pdl_entry();
     constexpr int kLanes = kCkptBlock / V;
-    constexpr int kU = V == 1 ? 8 : 4;
+    constexpr int kU = 32 / V;
     constexpr int kParts = GATED ? 2 : 1;
     constexpr bool kFast = Narrow<T>::value;
     const int lane = threadIdx.x % kLanes;
     const int64_t per_pass = int64_t(blockDim.x / kLanes);
-    int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
-    RowVec<T, V> in[kU][kParts], res[kU];
+    const int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
+    Chunk<T, V, ALIGNED> in[kU][kParts], res[kU];
     int64_t row[kU], blk[kU];
-    bool ok[kU];
+    int count[kU];  // elements of the row in this lane's chunk
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
         const int64_t u = u0 + i * per_pass;
-        ok[i] = u < p.units.count;
-        if (!ok[i]) continue;
+        count[i] = 0;
+        if (u >= p.units.count) continue;
         p.units.split(u, row[i], blk[i]);
         const int64_t col = blk[i] * kCkptBlock + lane * V;
-        ok[i] = col < p.n;
-        if (!ok[i]) continue;
+        count[i] = static_cast<int>(max(int64_t(0), min(int64_t(V), p.n - col)));
+        if (count[i] == 0) continue;
 #pragma unroll
-        for (int q = 0; q < kParts; ++q) in[i][q].load(p.z + row[i] * p.sz_m + q * p.sz_p + col);
-        if (p.residual != nullptr) res[i].load(p.residual + row[i] * p.sr_m + col);
+        for (int q = 0; q < kParts; ++q) in[i][q].load(p.z + row[i] * p.sz_m + q * p.sz_p + col, count[i]);
+        if (p.residual != nullptr) res[i].load(p.residual + row[i] * p.sr_m + col, count[i]);
     }
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
-        const int64_t u = u0 + i * per_pass;
-        const int64_t col = blk[i] * kCkptBlock + lane * V;
+        const bool in_range = u0 + i * per_pass < p.units.count;
+        const int64_t r = in_range ? row[i] : 0, b = in_range ? blk[i] : 0;
+        const int64_t col = b * kCkptBlock + lane * V;
         float z[kParts][V];
 #pragma unroll
         for (int q = 0; q < kParts; ++q) {
-            if (ok[i]) in[i][q].get(z[q]);
+            if (count[i] > 0) in[i][q].get(z[q]);
             else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) z[q][j] = 0.0f;
@@ -146,27 +203,26 @@ __global__ void __launch_bounds__(kThreads) ffn_forward_kernel(const ForwardPara
         if (p.values != nullptr) {
 #pragma unroll
             for (int q = 0; q < kParts; ++q) {
-                const bool in_range = u < p.units.count;
-                const int64_t at = in_range ? row[i] * kParts + q : 0;
-                pack_block<T, V>(z[q], ok[i] ? V : 0, lane, p.values + at * p.n + (ok[i] ? col : 0),
-                                 in_range ? p.exponents + at * p.units.nb + blk[i] : nullptr);
+                const int64_t at = r * kParts + q;
+                pack_block<T, V, ALIGNED>(z[q], count[i], lane, p.values + at * p.n + (count[i] > 0 ? col : 0),
+                                          in_range ? p.exponents + at * p.units.nb + b : nullptr);
             }
         }
-        if (p.y != nullptr && ok[i]) {
+        if (p.y != nullptr && count[i] > 0) {
             act_values<kFast, V>(p.act, z[0]);
             if constexpr (GATED) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) z[0][j] *= z[1][j];
             }
             if (p.residual != nullptr) {
-                float r[V];
-                res[i].get(r);
+                float t[V];
+                res[i].get(t);
 #pragma unroll
-                for (int j = 0; j < V; ++j) z[0][j] += r[j];
+                for (int j = 0; j < V; ++j) z[0][j] += t[j];
             }
-            RowVec<T, V> out;
+            Chunk<T, V, ALIGNED> out;
             out.set(z[0]);
-            out.store(p.y + row[i] * p.sy_m + col);
+            out.store(p.y + r * p.sy_m + col, count[i]);
         }
     }
 }
@@ -181,41 +237,38 @@ struct UnpackParams {
     Units units;
 };
 
-template <typename T, int V>
+template <typename T, int V, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const UnpackParams<T> p) {
     pdl_entry();
     constexpr int kLanes = kCkptBlock / V;
-    constexpr int kU = 4;
+    constexpr int kU = 32 / V;
     const int lane = threadIdx.x % kLanes;
     const int64_t per_pass = int64_t(blockDim.x / kLanes);
     const int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
-    Vec<int8_t, V> q[kU];
-    int stored[kU];
+    ByteChunk<V, ALIGNED> q[kU];
+    int stored[kU], count[kU];
     int64_t row[kU], col[kU];
-    bool ok[kU];
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
         const int64_t u = u0 + i * per_pass;
-        ok[i] = u < p.units.count;
-        if (!ok[i]) continue;
+        count[i] = 0;
+        if (u >= p.units.count) continue;
         int64_t blk;
         p.units.split(u, row[i], blk);
         col[i] = blk * kCkptBlock + lane * V;
-        ok[i] = col[i] < p.n;
-        if (!ok[i]) continue;
-        q[i] = *reinterpret_cast<const Vec<int8_t, V>*>(p.values + row[i] * p.n + col[i]);
+        count[i] = static_cast<int>(max(int64_t(0), min(int64_t(V), p.n - col[i])));
+        if (count[i] == 0) continue;
+        q[i].load(p.values + row[i] * p.n + col[i], count[i]);
         stored[i] = p.exponents[u];
     }
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
-        if (!ok[i]) continue;
-        const float step = ckpt_step(stored[i]);
+        if (count[i] == 0) continue;
         float f[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = float(q[i].v[j]) * step;
-        RowVec<T, V> out;
+        ckpt_values<V>(q[i].all(), stored[i], f);
+        Chunk<T, V, ALIGNED> out;
         out.set(f);
-        out.store(p.y + row[i] * p.sy_m + col[i]);
+        out.store(p.y + row[i] * p.sy_m + col[i], count[i]);
     }
 }
 
@@ -241,7 +294,7 @@ struct BackwardParams {
 // the fp32 sums of dz (before its rounding) over the block's rows.  A thread
 // keeps its V columns and walks the rows, so the sums stay in registers; they
 // are joined over the block in a fixed order and written as one partial row.
-template <typename T, int V, bool GATED, bool SAVED8>
+template <typename T, int V, bool GATED, bool SAVED8, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardParams<T> p) {
     pdl_entry();
     constexpr int kParts = GATED ? 2 : 1;
@@ -252,31 +305,31 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
     const int ny = kThreads / p.tx;
     const int64_t col = (int64_t(blockIdx.x) * p.tx + tx) * V;
     const int64_t r1 = min(p.m, (int64_t(blockIdx.y) + 1) * p.rows_per_block);
-    const bool col_ok = col < p.n;
+    const int count = static_cast<int>(max(int64_t(0), min(int64_t(V), p.n - col)));
     float acc[kParts][V];
 #pragma unroll
     for (int q = 0; q < kParts; ++q) {
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[q][j] = 0.0f;
     }
-    if (col_ok) {
+    if (count > 0) {
         for (int64_t r = int64_t(blockIdx.y) * p.rows_per_block + ty; r < r1; r += int64_t(ny) * kU) {
-            RowVec<T, V> dyv[kU], zv[kU][kParts];
-            Vec<int8_t, V> qv[kU][kParts];
+            Chunk<T, V, ALIGNED> dyv[kU], zv[kU][kParts];
+            ByteChunk<V, ALIGNED> qv[kU][kParts];
             int ev[kU][kParts];
 #pragma unroll
             for (int i = 0; i < kU; ++i) {
                 const int64_t row = r + int64_t(i) * ny;
                 if (row >= r1) continue;
-                dyv[i].load(p.dy + row * p.sdy_m + col);
+                dyv[i].load(p.dy + row * p.sdy_m + col, count);
 #pragma unroll
                 for (int q = 0; q < kParts; ++q) {
                     if constexpr (SAVED8) {
                         const int64_t at = row * kParts + q;
-                        qv[i][q] = *reinterpret_cast<const Vec<int8_t, V>*>(p.values + at * p.n + col);
+                        qv[i][q].load(p.values + at * p.n + col, count);
                         ev[i][q] = p.exponents[at * p.nb + col / kCkptBlock];
                     } else {
-                        zv[i][q].load(p.z + row * p.sz_m + q * p.sz_p + col);
+                        zv[i][q].load(p.z + row * p.sz_m + q * p.sz_p + col, count);
                     }
                 }
             }
@@ -289,15 +342,13 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
 #pragma unroll
                 for (int q = 0; q < kParts; ++q) {
                     if constexpr (SAVED8) {
-                        const float step = ckpt_step(ev[i][q]);
-#pragma unroll
-                        for (int j = 0; j < V; ++j) z[q][j] = float(qv[i][q].v[j]) * step;
+                        ckpt_values<V>(qv[i][q].all(), ev[i][q], z[q]);
                     } else {
                         zv[i][q].get(z[q]);
                     }
                 }
                 act_slopes<kFast, V>(p.act, z[0], a, d);
-                RowVec<T, V> out;
+                Chunk<T, V, ALIGNED> out;
                 if constexpr (GATED) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
@@ -306,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
                         dy[j] *= z[1][j];
                     }
                     out.set(a);
-                    out.store(p.dz + row * p.sdz_m + p.sdz_p + col);
+                    out.store(p.dz + row * p.sdz_m + p.sdz_p + col, count);
                 }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -314,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
                     acc[0][j] += d[j];
                 }
                 out.set(d);
-                out.store(p.dz + row * p.sdz_m + col);
+                out.store(p.dz + row * p.sdz_m + col, count);
             }
         }
     }
@@ -457,19 +508,22 @@ unsigned unit_blocks(const Units& u, int lanes, int unroll) {
 
 template <typename T, bool GATED>
 void launch_forward(ForwardParams<T>& p, cudaStream_t s) {
-    const bool vec = p.n % 8 == 0 && rows16(p.z, p.sz_m, sizeof(T)) && rows16(p.z, p.sz_p, sizeof(T)) &&
-                     rows16(p.residual, p.sr_m, sizeof(T)) && rows16(p.y, p.sy_m, sizeof(T)) &&
-                     reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
-    if (vec) {
-        launch_pdl(ffn_forward_kernel<T, 8, GATED>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
+    const bool aligned = p.n % 8 == 0 && rows16(p.z, p.sz_m, sizeof(T)) && rows16(p.z, p.sz_p, sizeof(T)) &&
+                         rows16(p.residual, p.sr_m, sizeof(T)) && rows16(p.y, p.sy_m, sizeof(T)) &&
+                         reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    if (aligned && !GATED && p.n % 16 == 0 && aligned16(p.values)) {
+        launch_pdl(ffn_forward_kernel<T, GATED ? 8 : 16, GATED, kAligned>, unit_blocks(p.units, 2, 2), kThreads, 0, s, p);
+    } else if (aligned) {
+        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAligned>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
     } else {
-        launch_pdl(ffn_forward_kernel<T, 1, GATED>, unit_blocks(p.units, 32, 8), kThreads, 0, s, p);
+        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAnywhere>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
     }
     check_launch("ffn_forward");
 }
 
-template <typename T, int V, bool GATED, bool SAVED8>
+template <typename T, bool GATED, bool SAVED8, bool ALIGNED>
 void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaStream_t s) {
+    constexpr int V = 8;
     // Threads along the columns: enough for one row, at most the block.
     int tx = 1;
     while (tx < kThreads && int64_t(tx) * V < p.n) tx <<= 1;
@@ -486,7 +540,7 @@ void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaSt
     }
     p.rows_per_block = (p.m + gy - 1) / gy;
     TPB_CHECK(gx < (int64_t(1) << 31), "activation_backward: too many columns");
-    launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8>, dim3(unsigned(gx), unsigned(gy)), kThreads, 0, s, p);
+    launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, ALIGNED>, dim3(unsigned(gx), unsigned(gy)), kThreads, 0, s, p);
     check_launch("ffn_backward");
 }
 
@@ -496,11 +550,11 @@ void dispatch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cuda
                      rows16(p.z, p.sz_p, sizeof(T)) && rows16(p.dz, p.sdz_m, sizeof(T)) &&
                      rows16(p.dz, p.sdz_p, sizeof(T)) && reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
     if (p.values != nullptr) {
-        if (vec) launch_backward<T, 8, GATED, true>(p, partial_rows, dev, s);
-        else launch_backward<T, 1, GATED, true>(p, partial_rows, dev, s);
+        if (vec) launch_backward<T, GATED, true, kAligned>(p, partial_rows, dev, s);
+        else launch_backward<T, GATED, true, kAnywhere>(p, partial_rows, dev, s);
     } else {
-        if (vec) launch_backward<T, 8, GATED, false>(p, partial_rows, dev, s);
-        else launch_backward<T, 1, GATED, false>(p, partial_rows, dev, s);
+        if (vec) launch_backward<T, GATED, false, kAligned>(p, partial_rows, dev, s);
+        else launch_backward<T, GATED, false, kAnywhere>(p, partial_rows, dev, s);
     }
 }
 
@@ -716,10 +770,13 @@ int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, con
             p.exponents = static_cast<const uint8_t*>(exponents->data);
             p.n = n;
             p.units = make_units(m, n);
-            if (n % 8 == 0 && rows16(p.y, p.sy_m, sizeof(scalar_t)) && reinterpret_cast<uintptr_t>(p.values) % 8 == 0) {
-                launch_pdl(checkpoint_unpack_kernel<scalar_t, 8>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
+            const bool vec = rows16(p.y, p.sy_m, sizeof(scalar_t));
+            if (vec && n % 16 == 0 && aligned16(p.values)) {
+                launch_pdl(checkpoint_unpack_kernel<scalar_t, 16, kAligned>, unit_blocks(p.units, 2, 2), kThreads, 0, s, p);
+            } else if (vec && n % 8 == 0 && reinterpret_cast<uintptr_t>(p.values) % 8 == 0) {
+                launch_pdl(checkpoint_unpack_kernel<scalar_t, 8, kAligned>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
             } else {
-                launch_pdl(checkpoint_unpack_kernel<scalar_t, 1>, unit_blocks(p.units, 32, 4), kThreads, 0, s, p);
+                launch_pdl(checkpoint_unpack_kernel<scalar_t, 8, kAnywhere>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
             }
             check_launch("checkpoint_unpack");
         });

@@ -109,11 +109,11 @@ __device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_
             for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             float qmax;
             const int stored = ckpt_exponent<T>(amax, qmax);
-            const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+            const Vec<int8_t, V> packed = ckpt_quantise<V>(z[q], stored, qmax);
             const int64_t row = m * PARTS + q;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if (j < left) f.values[row * p.N + n + j] = ckpt_quantise(z[q][j], inverse, qmax);
+                if (j < left) f.values[row * p.N + n + j] = packed.v[j];
             }
             if (n % kCkptBlock == 0 && left > 0) f.exponents[row * f.nb + n / kCkptBlock] = static_cast<uint8_t>(stored);
         }

@@ -51,13 +51,11 @@ __device__ __forceinline__ uint8_t stage_checkpoint(uint8_t* stage, int lane, co
     for (int j = 0; j < 32; ++j) amax = max_nan(amax, fabsf(z[j]));
     float qmax;
     const int stored = ckpt_exponent<T>(amax, qmax);
-    const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
+    const Vec<int8_t, 32> q = ckpt_quantise<32>(z, stored, qmax);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        Vec<int8_t, 16> q;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) q.v[j] = ckpt_quantise(z[h * 16 + j], inverse, qmax);
-        *reinterpret_cast<Vec<int8_t, 16>*>(stage + stage_offset(1, lane, h * 16)) = q;
+        *reinterpret_cast<Vec<int8_t, 16>*>(stage + stage_offset(1, lane, h * 16)) =
+            reinterpret_cast<const Vec<int8_t, 16>*>(&q)[h];
     }
     return static_cast<uint8_t>(stored);
 }
