@@ -66,6 +66,28 @@ __device__ __forceinline__ void act_slope(float z, float& a, float& d) {
 // more than the memory traffic of these passes (gelu's slope: 222 us over
 // 8192 x 16384 bf16 from 8 bits, against 103 us for the bytes).
 
+// a <- a * b and a <- a + b.
+template <int V>
+__device__ __forceinline__ void mul_to(float (&a)[V], const float (&b)[V]) {
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) {
+        const float2 r = __fmul2_rn(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]));
+        a[j] = r.x;
+        a[j + 1] = r.y;
+    }
+    if constexpr (V % 2) a[V - 1] *= b[V - 1];
+}
+template <int V>
+__device__ __forceinline__ void add_to(float (&a)[V], const float (&b)[V]) {
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) {
+        const float2 r = __fadd2_rn(make_float2(a[j], a[j + 1]), make_float2(b[j], b[j + 1]));
+        a[j] = r.x;
+        a[j + 1] = r.y;
+    }
+    if constexpr (V % 2) a[V - 1] += b[V - 1];
+}
+
 // 1 / (1 + 2^t): exp2 overflowing to infinity gives 0.
 __device__ __forceinline__ float2 gate_of_exp2(float2 t) {
     float2 e, r;
@@ -230,13 +252,22 @@ __device__ __forceinline__ float ckpt_step(int stored) {
 template <int V>
 __device__ __forceinline__ Vec<int8_t, V> ckpt_quantise(const float (&x)[V], int stored, float qmax) {
     const float inverse = stored == kCkptNonFinite ? 0.0f : ckpt_inverse(stored);
-    uint32_t bits[V];
+    float q[V], scale[V], round[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float q = x[j] * inverse;
-        if (qmax < 127.0f) q = fminf(fmaxf(q, -qmax), qmax);  // one block in a type's last binade; NaN * 0 = 0
-        bits[j] = __float_as_uint(q + 12582912.0f);
+        q[j] = x[j];
+        scale[j] = inverse;
+        round[j] = 12582912.0f;
     }
+    mul_to<V>(q, scale);
+    if (qmax < 127.0f) {  // a block in the type's last binade, or one that is not finite (NaN becomes 0)
+#pragma unroll
+        for (int j = 0; j < V; ++j) q[j] = fminf(fmaxf(q[j], -qmax), qmax);
+    }
+    add_to<V>(q, round);
+    uint32_t bits[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) bits[j] = __float_as_uint(q[j]);
     Vec<int8_t, V> out;
     if constexpr (V % 4 == 0) {
         uint32_t* o = reinterpret_cast<uint32_t*>(&out);
@@ -264,8 +295,12 @@ __device__ __forceinline__ void ckpt_values(const Vec<int8_t, V>& q, int stored,
         for (int j = 0; j < V; j += 4) {
             const uint32_t u = w[j / 4] ^ 0x80808080u;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                x[j + b] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + b)) - 8388736.0f) * step;
+            for (int b = 0; b < 4; b += 2) {
+                const float2 v = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + b)),
+                                             __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541 + b)));
+                const float2 r = __fmul2_rn(__fadd2_rn(v, f2(-8388736.0f)), f2(step));
+                x[j + b] = r.x;
+                x[j + b + 1] = r.y;
             }
         }
     } else {

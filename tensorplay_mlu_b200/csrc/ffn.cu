@@ -122,14 +122,34 @@ Units make_units(int64_t rows, int64_t n) {
     return u;
 }
 
-// One block's values and exponent, from V elements in each of its lanes (zero
-// past the row's end; `count` of them exist).
+// The largest magnitude of a chunk's elements (NaN if one is); 16-bit floats
+// are compared two at a time as they lie.
 template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void pack_block(const float (&x)[V], int count, int lane_in_block, int8_t* values,
-                                           uint8_t* exponent) {
-    float amax = 0.0f;
+__device__ __forceinline__ float largest(const Chunk<T, V, ALIGNED>& c) {
+    using C = Chunk<T, V, ALIGNED>;
+    if constexpr (sizeof(T) == 2) {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2* p = reinterpret_cast<const T2*>(&c.part);
+        T2 m = __habs2(p[0]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) amax = max_nan(amax, fabsf(x[j]));
+        for (int j = 1; j < V / 2; ++j) m = __hmax2_nan(m, __habs2(p[j]));
+        return max_nan(load_as<float>(m.x), load_as<float>(m.y));
+    } else {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V / C::kPer; ++i) {
+#pragma unroll
+            for (int j = 0; j < C::kPer; ++j) m = max_nan(m, fabsf(c.part[i].v[j]));
+        }
+        return m;
+    }
+}
+
+// One block's values and exponent, from V elements in each of its lanes and
+// their largest magnitude (zero past the row's end; `count` of them exist).
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void pack_block(const float (&x)[V], float amax, int count, int lane_in_block,
+                                           int8_t* values, uint8_t* exponent) {
 #pragma unroll
     for (int o = 1; o < kCkptBlock / V; o <<= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     float qmax;
@@ -159,12 +179,12 @@ struct ForwardParams {
 
 // y = act(z0) [* z1] [+ residual] and the checkpoint of z0 [and z1]; a thread
 // holds V elements of a unit, kU units at a time so that their loads are in
-// flight together.
-template <typename T, int V, bool GATED, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) ffn_forward_kernel(const ForwardParams<T> p) {
+// flight together.  PACK: the checkpoint alone.
+template <typename T, int V, bool GATED, bool ALIGNED, bool PACK>
+__global__ void __launch_bounds__(kThreads, 4) ffn_forward_kernel(const ForwardParams<T> p) {
     pdl_entry();
     constexpr int kLanes = kCkptBlock / V;
-    constexpr int kU = 32 / V;
+    constexpr int kU = (sizeof(T) == 4 || GATED ? 16 : 32) / V;
     constexpr int kParts = GATED ? 2 : 1;
     constexpr bool kFast = Narrow<T>::value;
     const int lane = threadIdx.x % kLanes;
@@ -184,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) ffn_forward_kernel(const ForwardPara
         if (count[i] == 0) continue;
 #pragma unroll
         for (int q = 0; q < kParts; ++q) in[i][q].load(p.z + row[i] * p.sz_m + q * p.sz_p + col, count[i]);
-        if (p.residual != nullptr) res[i].load(p.residual + row[i] * p.sr_m + col, count[i]);
+        if (!PACK && p.residual != nullptr) res[i].load(p.residual + row[i] * p.sr_m + col, count[i]);
     }
 #pragma unroll
     for (int i = 0; i < kU; ++i) {
@@ -200,15 +220,15 @@ __global__ void __launch_bounds__(kThreads) ffn_forward_kernel(const ForwardPara
                 for (int j = 0; j < V; ++j) z[q][j] = 0.0f;
             }
         }
-        if (p.values != nullptr) {
+        if (PACK || p.values != nullptr) {
 #pragma unroll
             for (int q = 0; q < kParts; ++q) {
                 const int64_t at = r * kParts + q;
-                pack_block<T, V, ALIGNED>(z[q], count[i], lane, p.values + at * p.n + (count[i] > 0 ? col : 0),
+                pack_block<T, V, ALIGNED>(z[q], count[i] > 0 ? largest(in[i][q]) : 0.0f, count[i], lane, p.values + at * p.n + (count[i] > 0 ? col : 0),
                                           in_range ? p.exponents + at * p.units.nb + b : nullptr);
             }
         }
-        if (p.y != nullptr && count[i] > 0) {
+        if (!PACK && p.y != nullptr && count[i] > 0) {
             act_values<kFast, V>(p.act, z[0]);
             if constexpr (GATED) {
 #pragma unroll
@@ -290,15 +310,22 @@ struct BackwardParams {
     int tx;  // threads along the columns (a power of two)
 };
 
+// Rows a thread loads before it computes: with four blocks an SM (64 registers)
+// one or two of them keep 48 to 64 KB in flight.
+template <typename T, bool GATED>
+__host__ __device__ constexpr int rows_at_once() {
+    return GATED || sizeof(T) == 4 ? 1 : 2;
+}
+
 // dz0 = dy [* z1] act'(z0) [, dz1 = dy act(z0)] and, for the bias gradient,
 // the fp32 sums of dz (before its rounding) over the block's rows.  A thread
 // keeps its V columns and walks the rows, so the sums stay in registers; they
 // are joined over the block in a fixed order and written as one partial row.
-template <typename T, int V, bool GATED, bool SAVED8, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardParams<T> p) {
+template <typename T, int V, bool GATED, bool SAVED8, bool ALIGNED, bool SUMS>
+__global__ void __launch_bounds__(kThreads, 4) ffn_backward_kernel(const BackwardParams<T> p) {
     pdl_entry();
     constexpr int kParts = GATED ? 2 : 1;
-    constexpr int kU = GATED ? 2 : 4;
+    constexpr int kU = rows_at_once<T, GATED>();
     constexpr bool kFast = Narrow<T>::value;
     const int tx = threadIdx.x & (p.tx - 1);
     const int ty = threadIdx.x / p.tx;
@@ -350,26 +377,20 @@ __global__ void __launch_bounds__(kThreads) ffn_backward_kernel(const BackwardPa
                 act_slopes<kFast, V>(p.act, z[0], a, d);
                 Chunk<T, V, ALIGNED> out;
                 if constexpr (GATED) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        a[j] *= dy[j];
-                        acc[1][j] += a[j];
-                        dy[j] *= z[1][j];
-                    }
+                    mul_to<V>(a, dy);
+                    if constexpr (SUMS) add_to<V>(acc[1], a);
+                    mul_to<V>(dy, z[1]);
                     out.set(a);
                     out.store(p.dz + row * p.sdz_m + p.sdz_p + col, count);
                 }
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    d[j] *= dy[j];
-                    acc[0][j] += d[j];
-                }
+                mul_to<V>(d, dy);
+                if constexpr (SUMS) add_to<V>(acc[0], d);
                 out.set(d);
                 out.store(p.dz + row * p.sdz_m + col, count);
             }
         }
     }
-    if (p.partial == nullptr) return;
+    if constexpr (!SUMS) return;
     __shared__ float sums[kThreads * V];
 #pragma unroll
     for (int q = 0; q < kParts; ++q) {
@@ -508,15 +529,22 @@ unsigned unit_blocks(const Units& u, int lanes, int unroll) {
 
 template <typename T, bool GATED>
 void launch_forward(ForwardParams<T>& p, cudaStream_t s) {
+    constexpr int per = sizeof(T) == 4 || GATED ? 16 : 32;  // elements a thread holds
     const bool aligned = p.n % 8 == 0 && rows16(p.z, p.sz_m, sizeof(T)) && rows16(p.z, p.sz_p, sizeof(T)) &&
                          rows16(p.residual, p.sr_m, sizeof(T)) && rows16(p.y, p.sy_m, sizeof(T)) &&
                          reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
-    if (aligned && !GATED && p.n % 16 == 0 && aligned16(p.values)) {
-        launch_pdl(ffn_forward_kernel<T, GATED ? 8 : 16, GATED, kAligned>, unit_blocks(p.units, 2, 2), kThreads, 0, s, p);
+    if (!GATED && p.y == nullptr) {
+        if (aligned && p.n % 16 == 0 && aligned16(p.values)) {
+            launch_pdl(ffn_forward_kernel<T, 16, false, kAligned, true>, unit_blocks(p.units, 2, per / 16), kThreads, 0, s, p);
+        } else if (aligned) {
+            launch_pdl(ffn_forward_kernel<T, 8, false, kAligned, true>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
+        } else {
+            launch_pdl(ffn_forward_kernel<T, 8, false, kAnywhere, true>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
+        }
     } else if (aligned) {
-        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAligned>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
+        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAligned, false>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
     } else {
-        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAnywhere>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
+        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAnywhere, false>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
     }
     check_launch("ffn_forward");
 }
@@ -534,13 +562,15 @@ void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaSt
         gy = partial_rows;
     } else {
         // About eight blocks an SM, and no more than one pass of rows needs.
-        const int64_t pass = int64_t(kThreads / tx) * (GATED ? 2 : 4);
+        const int64_t pass = int64_t(kThreads / tx) * rows_at_once<T, GATED>();
         gy = std::max<int64_t>(1, std::min<int64_t>((p.m + pass - 1) / pass, (int64_t(num_sms(dev)) * 8 + gx - 1) / gx));
         gy = std::min<int64_t>(gy, 65535);
     }
     p.rows_per_block = (p.m + gy - 1) / gy;
     TPB_CHECK(gx < (int64_t(1) << 31), "activation_backward: too many columns");
-    launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, ALIGNED>, dim3(unsigned(gx), unsigned(gy)), kThreads, 0, s, p);
+    const dim3 grid{unsigned(gx), unsigned(gy), 1};
+    if (p.partial != nullptr) launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, ALIGNED, true>, grid, kThreads, 0, s, p);
+    else launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, ALIGNED, false>, grid, kThreads, 0, s, p);
     check_launch("ffn_backward");
 }
 
