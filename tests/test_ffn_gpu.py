@@ -123,10 +123,13 @@ def activation_bound(z, e):
 SHAPES = [(1, 64, 32), (1, 4096, 1000), (3, 1027, 129), (17, 256, 96), (33, 512, 4099), (64, 96, 640),
           (129, 200, 264), (255, 72, 1000), (300, 520, 1032), (513, 1000, 777), (1030, 64, 1536), (2, 1, 1),
           (65, 8, 7)]
+# A wide weight for one and a few rows (tiles of 128 + 128 columns), more rows
+# than one tile of 64 or 128 with K split over a cluster.
+WIDE = [(1, 768, 11008), (24, 256, 11008), (100, 2048, 520), (200, 4096, 96), (600, 512, 1032)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("shape", SHAPES + WIDE)
 def test_gated_linear_forward(ops, dtype, shape):
     m, k, n = shape
     u = half_eps(dtype)
@@ -158,7 +161,7 @@ def test_gated_linear_forward(ops, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("shape", SHAPES + WIDE)
 def test_linear_act_forward(ops, dtype, shape):
     m, k, n = shape
     u = half_eps(dtype)
@@ -422,6 +425,111 @@ def test_empty_sizes(ops, dtype):
     assert dx.shape == (3, 0) and dw.shape == (32, 0) and db.shape == (32,)
     v, x = ops.checkpoint_pack(e(4, 0))
     assert ops.checkpoint_unpack(v, x, dtype).shape == (4, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [3, 140])
+def test_infinities_and_nan_go_where_arithmetic_puts_them(ops, dtype, m):
+    """A row of x or of the weight with an infinity or a NaN gives the
+    infinities and NaN of a plain sum, and leaves the other results alone; so
+    do values near the type's largest, whose products overflow."""
+    k, n = 200, 136
+    x, w = rand(m, k, dtype=dtype, seed=1), rand(n, k, dtype=dtype, seed=2, scale=k ** -0.5)
+    x[0, 3] = math.inf
+    x[1, 150] = -math.inf
+    x[2, 7], x[2, 8] = math.inf, -math.inf
+    w[5, 3] = 0.0            # inf * 0
+    w[9, 60] = math.nan
+    w[17, 70] = math.inf
+    z = x.float().double() @ w.float().double().t()
+    y, pre = ops.native_linear_act(dev(x), dev(w), None, None, "relu")
+    want = torch.where(torch.isnan(z), z, z.clamp_min(0))
+    for got, ref in ((pre, z), (y, want)):
+        got = got.cpu().double()
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.isinf(got), torch.isinf(ref))
+        assert torch.equal(got[torch.isinf(ref)], ref[torch.isinf(ref)])
+        fine = torch.isfinite(ref)
+        bound = (k + 8) * 2.0 ** -23 * 200 + half_eps(dtype) * (ref.abs() + 1) * 2
+        assert bool(((got - ref).abs() <= bound)[fine].all())
+    # gradients: dx rows of an infinite dy, dw columns of an infinite x
+    dy = rand(m, n, dtype=dtype, seed=3, scale=0.1)
+    dy[0, 0] = math.inf
+    saved = torch.ones(m, n, dtype=dtype)
+    dx, dw, db = ops.native_linear_act_backward(dev(dy), dev(x), dev(w), dev(saved), "none")
+    for got, ref in ((dx, dy.double() @ w.double()), (dw, dy.double().t() @ x.double()), (db, dy.double().sum(0))):
+        got = got.cpu().double()
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.isinf(got), torch.isinf(ref))
+    if dtype == torch.float32:
+        big = torch.full((m, 4), torch.finfo(dtype).max, dtype=dtype)
+        got = ops.linear_act(dev(big), dev(torch.eye(4, dtype=dtype)))
+        assert torch.equal(got.cpu(), big)   # a value that rounds past the largest TF32
+        # the checkpoint of a row with an infinity
+    h, (v, e) = ops.native_linear_act(dev(x), dev(w), None, None, "none", checkpoint=True)
+    back = ops.checkpoint_unpack(v, e, torch.float32).cpu()
+    blocks = torch.nn.functional.pad(z, (0, -n % 32)).unflatten(1, (-1, 32))
+    bad = (~torch.isfinite(blocks)).any(-1, keepdim=True).expand_as(blocks).flatten(1)[:, :n]
+    assert torch.equal(torch.isnan(back), bad)
+
+
+def test_offsets_past_32_bits(ops):
+    """Results of more than 2^31 elements, checked on rows at both ends."""
+    m, k, n = 98304, 64, 11008
+    assert 2 * m * n > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(m, k, generator=g, device="cuda", dtype=torch.float32).bfloat16()
+    w = dev(rand(2 * n, k, dtype=torch.bfloat16, seed=2, scale=k ** -0.5))
+    h, gate_up = ops.native_gated_linear(x, w)
+    rows = torch.tensor([0, 1, 48777, 97999, 98302, 98303], device="cuda")
+    z = x[rows].double() @ w.double().t()
+    u = half_eps(torch.bfloat16)
+    bound = (k + 8) * 2.0 ** -23 * (x[rows].double().abs() @ w.double().abs().t()) + u * z.abs() + 1e-30
+    assert bool(((gate_up[rows].flatten(1).double() - z).abs() <= bound).all())
+    held = ops.checkpoint_pack(gate_up)
+    for r in rows.tolist():
+        v, e, _ = pack_reference(gate_up[r].cpu())
+        assert torch.equal(held[0][r].cpu(), v) and torch.equal(held[1][r].cpu(), e)
+    del h
+    dy = torch.ones(m, n, device="cuda", dtype=torch.bfloat16)
+    dx, _, db = ops.native_gated_linear_backward(dy, x, w, held, "none", (True, False, True))
+    del held
+    packed = ops.checkpoint_pack(gate_up[rows])
+    part, _, _ = ops.native_gated_linear_backward(dy[:6], x[rows], w, packed, "none", (True, False, False))
+    scale = part.double().abs().max()
+    assert bool(((dx[rows].double() - part.double()).abs() <= 2.0 ** -6 * scale).all())
+
+
+def test_first_call_in_a_recording(backend):
+    """A process whose first feed-forward calls are recorded, without a warm-up."""
+    import subprocess
+    import sys
+
+    script = """
+import torch, tensorplay_mlu_b200 as tpb
+tpb.load()
+from tensorplay_mlu_b200.graph import Graph
+ops = tpb.ops
+torch.manual_seed(0)
+for dt in (torch.bfloat16, torch.float32):
+    for m in (2, 300):
+        x, w = torch.randn(m, 136).to(dt).cuda(), torch.randn(160, 136).to(dt).cuda()
+        def body():
+            h, s = ops.native_gated_linear(x, w)
+            return (h, *ops.native_gated_linear_backward(h, x, w, s))
+        g = Graph()
+        out = g.capture(body)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, body())), (dt, m)
+        del out
+        g.reset()
+assert tpb._native.lib().tp_b200_take_device_error(0) == 0
+print("recorded")
+"""
+    root = __import__("os").path.dirname(__import__("os").path.dirname(__import__("os").path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, cwd=root, timeout=300)
+    assert done.returncode == 0 and "recorded" in done.stdout, done.stderr[-2000:]
 
 
 def test_refusals(ops):
