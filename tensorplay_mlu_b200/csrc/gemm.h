@@ -57,7 +57,8 @@ struct FfnProblem {
     int flags;
 };
 
-// 16-bit floats: sx_k 1; sw_k 1, or sw_n 1 without an epilogue.  False when x
+// 16-bit floats: sx_k and sw_k 1; or, without an epilogue, sw_n 1 (dz w), or
+// sx_m and sw_n 1 (dz^T x).  False when x
 // or w does not fit the tensor maps (rows off 16-byte boundaries) or K is 0;
 // nothing has been launched then.
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream);

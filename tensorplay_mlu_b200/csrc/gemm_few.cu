@@ -19,7 +19,9 @@
 //     order (the same bits on every run, no workspace, no atomics), then
 //     applies bias, activation, gate and residual in fp32.
 // The weight is read K-major (x W^T) or, for the input gradient dz W, in
-// place as an MN-major operand.
+// place as an MN-major operand.  The weight gradient dz^T x of many rows and
+// few features has the same shape of problem (a long sum, few tiles); there
+// both operands are MN-major.
 //
 // Every wait is bounded as in gemm_tc.cu; all threads reach the cluster
 // barriers.  No TMA multicast is used.
@@ -48,7 +50,7 @@ struct FewShape {
     static constexpr int kTmemCols = WT * NT < 32 ? 32 : WT * NT;  // a power of two
 };
 
-template <typename T, int PARTS, int NT, int WT, bool W_MN>
+template <typename T, int PARTS, int NT, int WT, bool W_MN, bool X_MN>
 __global__ void __launch_bounds__(kFewThreads)
     gemm_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const FewParams p) {
     using S = FewShape<NT, WT>;
@@ -111,7 +113,8 @@ __global__ void __launch_bounds__(kFewThreads)
                     load_operand<2, W_MN, false, false>(at + q * (S::kWBytes / PARTS), &tmW, fb, n0 + q * p.N, kb * 64,
                                                         0, kColumns);
                 }
-                tma_load_2d(at + S::kWBytes, &tmX, fb, kb * 64, m0);
+                if constexpr (X_MN) load_operand<2, true, false, false>(at + S::kWBytes, &tmX, fb, m0, kb * 64, 0, NT);
+                else tma_load_2d(at + S::kWBytes, &tmX, fb, kb * 64, m0);
                 if (++stage == kStages) {
                     stage = 0;
                     phase ^= 1;
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kFewThreads)
                 const uint32_t at = smem_addr(smem + stage * S::kStageBytes);
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t bd = sw128_desc(at + S::kWBytes + kk * 32, 16, 1024);
+                    const uint64_t bd = sw128_desc(at + S::kWBytes + kk * (X_MN ? 16 * 128 : 32), X_MN ? 8192 : 16, 1024);
 #pragma unroll
                     for (int t = 0; t < WT; ++t) {
                         const uint64_t ad = sw128_desc(at + t * 16384 + kk * a_kstep, a_lbo, 1024);
@@ -205,11 +208,11 @@ double stream_us(int64_t n, int64_t slots, double mb, int split) {
 }
 
 // Launches the product, or with `us` only estimates its time.
-template <typename T, int PARTS, int NT, int WT, bool W_MN>
+template <typename T, int PARTS, int NT, int WT, bool W_MN, bool X_MN>
 void launch_few(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
     using S = FewShape<NT, WT>;
-    auto kern = gemm_few_kernel<T, PARTS, NT, WT, W_MN>;
-    const Slots& slots = cluster_slots<gemm_few_kernel<T, PARTS, NT, WT, W_MN>>(kFewThreads, S::kSmem, dev);
+    auto kern = gemm_few_kernel<T, PARTS, NT, WT, W_MN, X_MN>;
+    const Slots& slots = cluster_slots<gemm_few_kernel<T, PARTS, NT, WT, W_MN, X_MN>>(kFewThreads, S::kSmem, dev);
     const int row_tiles = static_cast<int>((q.M + NT - 1) / NT), k_blocks = static_cast<int>((q.K + 63) / 64);
     const int64_t tiles = int64_t(row_tiles) * ((q.N + WT * 128 / PARTS - 1) / (WT * 128 / PARTS));
     int64_t waves = 1;
@@ -239,10 +242,13 @@ void launch_few(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStre
     }
     FewParams p = few_params(q, dev, 64);
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(W_MN) << 15) | (uint32_t(NT >> 3) << 17) |
+    p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (uint32_t(W_MN) << 15) | (uint32_t(X_MN) << 16) |
+              (uint32_t(NT >> 3) << 17) |
               (uint32_t(128 >> 4) << 24);
     p.row_tiles = row_tiles;
-    const CUtensorMap mx = make_map(q.x, type, 2, q.K, q.M, q.sx_m, 1, 0, NT);
+    static_assert(!X_MN || NT >= 64, "an MN-major operand is staged 64 rows at a time");
+    const CUtensorMap mx = X_MN ? make_map(q.x, type, 2, q.M, q.K, q.sx_k, 1, 0, 64)
+                                : make_map(q.x, type, 2, q.K, q.M, q.sx_m, 1, 0, NT);
     const CUtensorMap mw = W_MN ? make_map(q.w, type, 2, q.N, q.K, q.sw_k, 1, 0, 64)
                                 : make_map(q.w, type, 2, q.K, PARTS * q.N, q.sw_n, 1, 0, kBoxRows);
     launch_cluster(kern, tiles * split, split, kFewThreads, S::kSmem, stream, mw, mx, p);
@@ -255,13 +261,13 @@ template <typename T, int PARTS, int NT, bool W_MN>
 void launch_narrow(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
     if constexpr (PARTS == 2) {
         double one = 0.0, two = 0.0;
-        launch_few<T, PARTS, NT, 1, W_MN>(q, type, dev, stream, &one);
-        launch_few<T, PARTS, NT, 2, W_MN>(q, type, dev, stream, &two);
+        launch_few<T, PARTS, NT, 1, W_MN, false>(q, type, dev, stream, &one);
+        launch_few<T, PARTS, NT, 2, W_MN, false>(q, type, dev, stream, &two);
         if (us != nullptr) *us = std::min(one, two);
-        else if (two < one) launch_few<T, PARTS, NT, 2, W_MN>(q, type, dev, stream, nullptr);
-        else launch_few<T, PARTS, NT, 1, W_MN>(q, type, dev, stream, nullptr);
+        else if (two < one) launch_few<T, PARTS, NT, 2, W_MN, false>(q, type, dev, stream, nullptr);
+        else launch_few<T, PARTS, NT, 1, W_MN, false>(q, type, dev, stream, nullptr);
     } else {
-        launch_few<T, PARTS, NT, 1, W_MN>(q, type, dev, stream, us);
+        launch_few<T, PARTS, NT, 1, W_MN, false>(q, type, dev, stream, us);
     }
 }
 
@@ -269,13 +275,16 @@ template <typename T, int PARTS, bool W_MN>
 void launch_rows(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
     if (q.M <= 16) launch_narrow<T, PARTS, 16, W_MN>(q, type, dev, stream, us);
     else if (q.M <= 32) launch_narrow<T, PARTS, 32, W_MN>(q, type, dev, stream, us);
-    else if (q.M <= 64) launch_few<T, PARTS, 64, 1, W_MN>(q, type, dev, stream, us);
-    else launch_few<T, PARTS, 128, 1, W_MN>(q, type, dev, stream, us);
+    else if (q.M <= 64) launch_few<T, PARTS, 64, 1, W_MN, false>(q, type, dev, stream, us);
+    else launch_few<T, PARTS, 128, 1, W_MN, false>(q, type, dev, stream, us);
 }
 
 template <typename T>
 void launch_typed(const FfnProblem& q, CUtensorMapDataType type, int dev, cudaStream_t stream, double* us) {
-    if (q.sw_k != 1) launch_rows<T, 1, true>(q, type, dev, stream, us);
+    if (q.sx_k != 1) {
+        if (q.M <= 64) launch_few<T, 1, 64, 1, true, true>(q, type, dev, stream, us);
+        else launch_few<T, 1, 128, 1, true, true>(q, type, dev, stream, us);
+    } else if (q.sw_k != 1) launch_rows<T, 1, true>(q, type, dev, stream, us);
     else if (q.parts == 2) launch_rows<T, 2, false>(q, type, dev, stream, us);
     else launch_rows<T, 1, false>(q, type, dev, stream, us);
 }

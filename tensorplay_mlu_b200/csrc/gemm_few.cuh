@@ -79,10 +79,23 @@ __device__ __forceinline__ uint32_t cluster_size() {
     return r;
 }
 
+// V elements of the residual of row m from column n on (zero without one).
+template <typename T, int V>
+__device__ __forceinline__ void load_residual(const FewParams& p, int64_t m, int64_t n, float (&r)[V]) {
+    const FfnParams& f = p.ffn;
+    if (f.residual != nullptr && n < p.N) {
+        load_few<T, V>(static_cast<const T*>(f.residual) + m * f.sres_m + n, p.N - n, r);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = 0.0f;
+    }
+}
+
 // V results of row m from column n on (a warp holds 32 V consecutive ones):
-// z[part] are their summed pre-activations.
+// z[part] are their summed pre-activations, r the residual.
 template <typename T, int PARTS, int V>
-__device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_t n, float (&z)[PARTS][V]) {
+__device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_t n, float (&z)[PARTS][V],
+                                           const float (&r)[V]) {
     const FfnParams& f = p.ffn;
     const int64_t left = p.N - n;  // may be negative
     const T* bias = static_cast<const T*>(f.bias);
@@ -124,12 +137,7 @@ __device__ __forceinline__ void finish_few(const FewParams& p, int64_t m, int64_
 #pragma unroll
         for (int j = 0; j < V; ++j) z[0][j] *= z[1][j];
     }
-    if (f.residual != nullptr) {
-        float r[V];
-        load_few<T, V>(static_cast<const T*>(f.residual) + m * f.sres_m + n, left, r);
-#pragma unroll
-        for (int j = 0; j < V; ++j) z[0][j] += r[j];
-    }
+    if (f.residual != nullptr) add_to<V>(z[0], r);
     store_few<T, V>(static_cast<T*>(p.y) + m * p.sy_m + n, left, z[0]);
 }
 
@@ -151,25 +159,39 @@ __device__ __forceinline__ void finish_rows(const FewParams& p, const float* par
     const int rows = min(NT, p.M - m0);
     const int64_t n = int64_t(n0) + lane * kV;
     if (ranks == 1) {
-        // Two rows at a time: their reads and the stores behind them overlap.
-#pragma unroll 2
-        for (int m = warp; m < rows; m += warps) {
-            float z[PARTS][kV];
+        // Four rows at a time, so that their reads are in flight together.
+        constexpr int kRows = 4;
+        for (int first = warp; first < rows; first += kRows * warps) {
+            float z[kRows][PARTS][kV], r[kRows][kV];
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) {
-                const Vec<float, kV> v = *reinterpret_cast<const Vec<float, kV>*>(partial + offset(m, q, lane));
+            for (int i = 0; i < kRows; ++i) {
+                const int m = first + i * warps;
+                if (m >= rows) break;
+                load_residual<T, kV>(p, int64_t(m0) + m, n, r[i]);
 #pragma unroll
-                for (int j = 0; j < kV; ++j) {
-                    z[q][j] = v.v[j];
-                    fix(int64_t(m0) + m, n + j, q, z[q][j]);
+                for (int q = 0; q < PARTS; ++q) {
+                    const Vec<float, kV> v = *reinterpret_cast<const Vec<float, kV>*>(partial + offset(m, q, lane));
+#pragma unroll
+                    for (int j = 0; j < kV; ++j) z[i][q][j] = v.v[j];
                 }
             }
-            finish_few<T, PARTS, kV>(p, int64_t(m0) + m, n, z);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int m = first + i * warps;
+                if (m >= rows) break;
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+#pragma unroll
+                    for (int j = 0; j < kV; ++j) fix(int64_t(m0) + m, n + j, q, z[i][q][j]);
+                }
+                finish_few<T, PARTS, kV>(p, int64_t(m0) + m, n, z[i], r[i]);
+            }
         }
         return;
     }
     for (int m = rank + ranks * warp; m < rows; m += ranks * warps) {
-        float z[PARTS][kV];
+        float z[PARTS][kV], r[kV];
+        load_residual<T, kV>(p, int64_t(m0) + m, n, r);
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
             const uint32_t at = smem_addr(partial + offset(m, q, lane));
@@ -192,7 +214,7 @@ __device__ __forceinline__ void finish_rows(const FewParams& p, const float* par
 #pragma unroll
             for (int j = 0; j < kV; ++j) fix(int64_t(m0) + m, n + j, q, z[q][j]);
         }
-        finish_few<T, PARTS, kV>(p, int64_t(m0) + m, n, z);
+        finish_few<T, PARTS, kV>(p, int64_t(m0) + m, n, z, r);
     }
 }
 

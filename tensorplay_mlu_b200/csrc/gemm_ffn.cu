@@ -275,7 +275,7 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
 // estimate here: 0.31 us for each 64-deep step of a wave of 256 x 256 tiles,
 // 2.2 us for a wave's ramp and epilogue, 5 us once.
 bool few_rows(const FfnProblem& q, int dev) {
-    if (q.M <= 64) return true;
+    if (q.M <= 64 && q.sx_k == 1) return true;
     const int64_t columns = q.parts == 2 ? 128 : kPairBN;
     const int64_t tiles = ((q.M + kPairBM - 1) / kPairBM) * ((q.N + columns - 1) / columns);
     const int64_t clusters = std::max(1, gemm_sm_budget(dev) / 2);
@@ -286,8 +286,8 @@ bool few_rows(const FfnProblem& q, int dev) {
 bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {
     const int64_t limit = int64_t(1) << 30;
     if (q.K == 0 || q.M >= limit || q.N >= limit || q.K >= limit) return false;
-    const bool transposed = q.sw_k != 1;
-    if (!tma_ok(q.x, 2, q.sx_m, 1, 0) || !tma_ok(q.w, 2, transposed ? q.sw_k : q.sw_n, 1, 0)) return false;
+    const bool transposed = q.sw_k != 1 || q.sx_k != 1;
+    if (!tma_ok(q.x, 2, q.sx_k != 1 ? q.sx_k : q.sx_m, 1, 0) || !tma_ok(q.w, 2, transposed ? q.sw_k : q.sw_n, 1, 0)) return false;
     TPB_CHECK(q.dtype == TPB_BF16 || q.dtype == TPB_F16, "feed-forward product: 16-bit floats only");
     if (few_rows(q, dev)) {
         gemm_few(q, dev, stream);
@@ -304,10 +304,10 @@ bool gemm_ffn(const FfnProblem& q, int dev, cudaStream_t stream) {
         p.batch = 1;
         p.a = q.x;
         p.sa_m = q.sx_m;
-        p.sa_k = 1;
+        p.sa_k = q.sx_k;
         p.b = q.w;
         p.sb_k = q.sw_k;
-        p.sb_n = 1;
+        p.sb_n = q.sw_n;
         p.c = q.y;
         p.sc_m = q.sy_m;
         p.alpha = 1.0;
