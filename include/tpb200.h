@@ -429,7 +429,7 @@ enum tpb_activation {
  * rounding at the end.  Matrices have unit column stride and the row strides
  * given (elements).
  *   x_work, w_work   16-byte-aligned workspaces of m (parts * n) rows of k
- *               elements rounded up to 16 bytes: x and w are copied there first
+ *               elements rounded up to 128 bytes: x and w are copied there first
  *               when their rows start off 16-byte boundaries.  bfloat16 and
  *               float16 need them then; float32 reads rows anywhere, and takes
  *               the copies only when given the workspaces (they pay where the

@@ -14,11 +14,13 @@ namespace tpb {
 namespace {
 
 // How a kernel's rows lie: kAligned, every chunk of V elements on a 16-byte
-// boundary (8 bytes for checkpoint values) and whole; or kAnywhere, in which
-// case chunks are read and written in the largest words they start on, and
-// a row's last one may be short.
-constexpr bool kAligned = true;
-constexpr bool kAnywhere = false;
+// boundary (8 bytes for checkpoint values) and whole; kWords, on a 4-byte
+// boundary, checkpoint values on a 2-byte one, a row's last chunk perhaps
+// short; kAnywhere, some rows half a word off.  (One kernel for the last two
+// took 1.3 to 1.7 times as long on rows of words.)
+constexpr int kAligned = 0;
+constexpr int kWords = 1;
+constexpr int kAnywhere = 2;
 
 // N bytes at p in words of W bytes (p a multiple of W).
 template <typename W, int N>
@@ -28,22 +30,35 @@ __device__ __forceinline__ void copy_in(void* to, const void* p) {
 }
 
 // V consecutive elements of E at p (`count` of them exist).
-template <typename E, int V, bool ALIGNED>
+template <typename E, int V, int MODE>
 struct Chunk {
     static constexpr int kBytes = V * int(sizeof(E));
     static constexpr int kPer = (16 < kBytes ? 16 : kBytes) / int(sizeof(E));
+    // Rows half a word off: pairs from the second element on lie on boundaries.
+    static constexpr bool kShifted = MODE == kAnywhere && sizeof(E) <= 2;
+    using Pair = typename std::conditional<sizeof(E) == 1, uint16_t, uint32_t>::type;
     Vec<E, kPer> part[V / kPer];
 
     __device__ __forceinline__ void load(const E* p, int count) {
-        if constexpr (ALIGNED) {
+        if constexpr (MODE == kAligned) {
 #pragma unroll
             for (int i = 0; i < V / kPer; ++i) part[i] = reinterpret_cast<const Vec<E, kPer>*>(p)[i];
         } else {
             const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-            if (count == V && at % 4 == 0) {
+            if (count == V && (at % 4 == 0 || (MODE == kWords && sizeof(E) > 1))) {
                 copy_in<uint32_t, kBytes>(part, p);
-            } else if (count == V && sizeof(E) == 1 && at % 2 == 0) {
+            } else if (count == V && sizeof(E) == 1 && (at % 2 == 0 || MODE == kWords)) {
                 copy_in<uint16_t, kBytes>(part, p);
+            } else if (count == V && kShifted) {
+                // One element, pairs of elements, one element.
+                E* e = reinterpret_cast<E*>(part);
+                e[0] = p[0];
+#pragma unroll
+                for (int j = 1; j + 2 < V; j += 2) {
+                    const Pair two = *reinterpret_cast<const Pair*>(p + j);
+                    memcpy(&e[j], &two, sizeof(Pair));
+                }
+                e[V - 1] = p[V - 1];
             } else {
                 E* e = reinterpret_cast<E*>(part);
 #pragma unroll
@@ -55,15 +70,25 @@ struct Chunk {
         }
     }
     __device__ __forceinline__ void store(E* p, int count) const {
-        if constexpr (ALIGNED) {
+        if constexpr (MODE == kAligned) {
 #pragma unroll
             for (int i = 0; i < V / kPer; ++i) reinterpret_cast<Vec<E, kPer>*>(p)[i] = part[i];
         } else {
             const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-            if (count == V && at % 4 == 0) {
+            if (count == V && (at % 4 == 0 || (MODE == kWords && sizeof(E) > 1))) {
                 copy_in<uint32_t, kBytes>(p, part);
-            } else if (count == V && sizeof(E) == 1 && at % 2 == 0) {
+            } else if (count == V && sizeof(E) == 1 && (at % 2 == 0 || MODE == kWords)) {
                 copy_in<uint16_t, kBytes>(p, part);
+            } else if (count == V && kShifted) {
+                const E* e = reinterpret_cast<const E*>(part);
+                p[0] = e[0];
+#pragma unroll
+                for (int j = 1; j + 2 < V; j += 2) {
+                    Pair two;
+                    memcpy(&two, &e[j], sizeof(Pair));
+                    *reinterpret_cast<Pair*>(p + j) = two;
+                }
+                p[V - 1] = e[V - 1];
             } else {
                 const E* e = reinterpret_cast<const E*>(part);
 #pragma unroll
@@ -94,8 +119,8 @@ struct Chunk {
 };
 
 // A checkpoint's int8 values, V of them.
-template <int V, bool ALIGNED>
-struct ByteChunk : Chunk<int8_t, V, ALIGNED> {
+template <int V, int MODE>
+struct ByteChunk : Chunk<int8_t, V, MODE> {
     __device__ __forceinline__ const Vec<int8_t, V>& all() const {
         static_assert(V <= 16, "one part");
         return this->part[0];
@@ -124,9 +149,9 @@ Units make_units(int64_t rows, int64_t n) {
 
 // The largest magnitude of a chunk's elements (NaN if one is); 16-bit floats
 // are compared two at a time as they lie.
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ float largest(const Chunk<T, V, ALIGNED>& c) {
-    using C = Chunk<T, V, ALIGNED>;
+template <typename T, int V, int MODE>
+__device__ __forceinline__ float largest(const Chunk<T, V, MODE>& c) {
+    using C = Chunk<T, V, MODE>;
     if constexpr (sizeof(T) == 2) {
         using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
         const T2* p = reinterpret_cast<const T2*>(&c.part);
@@ -147,7 +172,7 @@ __device__ __forceinline__ float largest(const Chunk<T, V, ALIGNED>& c) {
 
 // One block's values and exponent, from V elements in each of its lanes and
 // their largest magnitude (zero past the row's end; `count` of them exist).
-template <typename T, int V, bool ALIGNED>
+template <typename T, int V, int MODE>
 __device__ __forceinline__ void pack_block(const float (&x)[V], float amax, int count, int lane_in_block,
                                            int8_t* values, uint8_t* exponent) {
 #pragma unroll
@@ -155,7 +180,7 @@ __device__ __forceinline__ void pack_block(const float (&x)[V], float amax, int 
     float qmax;
     const int stored = ckpt_exponent<T>(amax, qmax);
     if (count > 0) {
-        Chunk<int8_t, V, ALIGNED> q;
+        Chunk<int8_t, V, MODE> q;
         q.part[0] = ckpt_quantise<V>(x, stored, qmax);
         q.store(values, count);
     }
@@ -180,7 +205,7 @@ struct ForwardParams {
 // y = act(z0) [* z1] [+ residual] and the checkpoint of z0 [and z1]; a thread
 // holds V elements of a unit, kU units at a time so that their loads are in
 // flight together.  PACK: the checkpoint alone.
-template <typename T, int V, bool GATED, bool ALIGNED, bool PACK>
+template <typename T, int V, bool GATED, int MODE, bool PACK>
 __global__ void __launch_bounds__(kThreads, 4) ffn_forward_kernel(const ForwardParams<T> p) {
     pdl_entry();
     constexpr int kLanes = kCkptBlock / V;
@@ -190,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 4) ffn_forward_kernel(const ForwardP
     const int lane = threadIdx.x % kLanes;
     const int64_t per_pass = int64_t(blockDim.x / kLanes);
     const int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
-    Chunk<T, V, ALIGNED> in[kU][kParts], res[kU];
+    Chunk<T, V, MODE> in[kU][kParts], res[kU];
     int64_t row[kU], blk[kU];
     int count[kU];  // elements of the row in this lane's chunk
 #pragma unroll
@@ -224,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 4) ffn_forward_kernel(const ForwardP
 #pragma unroll
             for (int q = 0; q < kParts; ++q) {
                 const int64_t at = r * kParts + q;
-                pack_block<T, V, ALIGNED>(z[q], count[i] > 0 ? largest(in[i][q]) : 0.0f, count[i], lane, p.values + at * p.n + (count[i] > 0 ? col : 0),
+                pack_block<T, V, MODE>(z[q], count[i] > 0 ? largest(in[i][q]) : 0.0f, count[i], lane, p.values + at * p.n + (count[i] > 0 ? col : 0),
                                           in_range ? p.exponents + at * p.units.nb + b : nullptr);
             }
         }
@@ -240,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 4) ffn_forward_kernel(const ForwardP
 #pragma unroll
                 for (int j = 0; j < V; ++j) z[0][j] += t[j];
             }
-            Chunk<T, V, ALIGNED> out;
+            Chunk<T, V, MODE> out;
             out.set(z[0]);
             out.store(p.y + r * p.sy_m + col, count[i]);
         }
@@ -257,7 +282,7 @@ struct UnpackParams {
     Units units;
 };
 
-template <typename T, int V, bool ALIGNED>
+template <typename T, int V, int MODE>
 __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const UnpackParams<T> p) {
     pdl_entry();
     constexpr int kLanes = kCkptBlock / V;
@@ -265,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const Unpac
     const int lane = threadIdx.x % kLanes;
     const int64_t per_pass = int64_t(blockDim.x / kLanes);
     const int64_t u0 = int64_t(blockIdx.x) * per_pass * kU + threadIdx.x / kLanes;
-    ByteChunk<V, ALIGNED> q[kU];
+    ByteChunk<V, MODE> q[kU];
     int stored[kU], count[kU];
     int64_t row[kU], col[kU];
 #pragma unroll
@@ -286,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) checkpoint_unpack_kernel(const Unpac
         if (count[i] == 0) continue;
         float f[V];
         ckpt_values<V>(q[i].all(), stored[i], f);
-        Chunk<T, V, ALIGNED> out;
+        Chunk<T, V, MODE> out;
         out.set(f);
         out.store(p.y + row[i] * p.sy_m + col[i], count[i]);
     }
@@ -326,7 +351,7 @@ __host__ __device__ constexpr int backward_blocks() {
 // the fp32 sums of dz (before its rounding) over the block's rows.  A thread
 // keeps its V columns and walks the rows, so the sums stay in registers; they
 // are joined over the block in a fixed order and written as one partial row.
-template <typename T, int V, bool GATED, bool SAVED8, bool ALIGNED, bool SUMS>
+template <typename T, int V, bool GATED, bool SAVED8, int MODE, bool SUMS>
 __global__ void __launch_bounds__(kThreads, (backward_blocks<T, GATED>())) ffn_backward_kernel(const BackwardParams<T> p) {
     pdl_entry();
     constexpr int kParts = GATED ? 2 : 1;
@@ -346,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, (backward_blocks<T, GATED>())) ffn_b
     }
     if (count > 0) {
         for (int64_t r = int64_t(blockIdx.y) * p.rows_per_block + ty; r < r1; r += int64_t(ny) * kU) {
-            Chunk<T, V, ALIGNED> dyv[kU], zv[kU][kParts];
-            ByteChunk<V, ALIGNED> qv[kU][kParts];
+            Chunk<T, V, MODE> dyv[kU], zv[kU][kParts];
+            ByteChunk<V, MODE> qv[kU][kParts];
             int ev[kU][kParts];
 #pragma unroll
             for (int i = 0; i < kU; ++i) {
@@ -380,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, (backward_blocks<T, GATED>())) ffn_b
                     }
                 }
                 act_slopes<kFast, V>(p.act, z[0], a, d);
-                Chunk<T, V, ALIGNED> out;
+                Chunk<T, V, MODE> out;
                 if constexpr (GATED) {
                     mul_to<V>(a, dy);
                     if constexpr (SUMS) add_to<V>(acc[1], a);
@@ -521,6 +546,10 @@ void require_checkpoint(const tpb_tensor* values, const tpb_tensor* exponents, c
     }
 }
 
+// Rows on 4-byte boundaries (checkpoint values of even rows: 2-byte ones).
+bool rows4(const void* p, int64_t pitch, size_t es) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 4 == 0 && (pitch * int64_t(es)) % 4 == 0);
+}
 // 16-byte vectors along n are possible for an operand of `es`-byte elements.
 bool rows16(const void* p, int64_t pitch, size_t es) {
     return p == nullptr || (aligned16(p) && (pitch * int64_t(es)) % 16 == 0);
@@ -535,31 +564,41 @@ unsigned unit_blocks(const Units& u, int lanes, int unroll) {
 template <typename T, bool GATED>
 void launch_forward(ForwardParams<T>& p, cudaStream_t s) {
     constexpr int per = sizeof(T) == 4 || GATED ? 16 : 32;  // elements a thread holds
-    const bool aligned = p.n % 8 == 0 && rows16(p.z, p.sz_m, sizeof(T)) && rows16(p.z, p.sz_p, sizeof(T)) &&
-                         rows16(p.residual, p.sr_m, sizeof(T)) && rows16(p.y, p.sy_m, sizeof(T)) &&
+    constexpr size_t es = sizeof(T);
+    const bool aligned = p.n % 8 == 0 && rows16(p.z, p.sz_m, es) && rows16(p.z, p.sz_p, es) &&
+                         rows16(p.residual, p.sr_m, es) && rows16(p.y, p.sy_m, es) &&
                          reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    const bool words = p.n % 2 == 0 && rows4(p.z, p.sz_m, es) && rows4(p.z, p.sz_p, es) &&
+                       rows4(p.residual, p.sr_m, es) && rows4(p.y, p.sy_m, es) &&
+                       reinterpret_cast<uintptr_t>(p.values) % 2 == 0;
+    const auto go = [&](auto kernel, int v) {
+        launch_pdl(kernel, unit_blocks(p.units, kCkptBlock / v, per / v), kThreads, 0, s, p);
+    };
     if (!GATED && p.y == nullptr) {
-        if (aligned && p.n % 16 == 0 && aligned16(p.values)) {
-            launch_pdl(ffn_forward_kernel<T, 16, false, kAligned, true>, unit_blocks(p.units, 2, per / 16), kThreads, 0, s, p);
-        } else if (aligned) {
-            launch_pdl(ffn_forward_kernel<T, 8, false, kAligned, true>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
-        } else {
-            launch_pdl(ffn_forward_kernel<T, 8, false, kAnywhere, true>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
-        }
+        if (aligned && p.n % 16 == 0 && aligned16(p.values)) go(ffn_forward_kernel<T, 16, false, kAligned, true>, 16);
+        else if (aligned) go(ffn_forward_kernel<T, 8, false, kAligned, true>, 8);
+        else if (words) go(ffn_forward_kernel<T, 8, false, kWords, true>, 8);
+        else go(ffn_forward_kernel<T, 8, false, kAnywhere, true>, 8);
     } else if (aligned) {
-        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAligned, false>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
+        go(ffn_forward_kernel<T, 8, GATED, kAligned, false>, 8);
     } else {
-        launch_pdl(ffn_forward_kernel<T, 8, GATED, kAnywhere, false>, unit_blocks(p.units, 4, per / 8), kThreads, 0, s, p);
+        go(ffn_forward_kernel<T, 8, GATED, kAnywhere, false>, 8);
     }
     check_launch("ffn_forward");
 }
 
-template <typename T, bool GATED, bool SAVED8, bool ALIGNED>
+template <typename T, bool GATED, bool SAVED8, int MODE>
 void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaStream_t s) {
     constexpr int V = 8;
     // Threads along the columns: enough for one row, at most the block.
     int tx = 1;
     while (tx < kThreads && int64_t(tx) * V < p.n) tx <<= 1;
+    // Where the partial sums fix the rows' split, narrower blocks until there
+    // are four for every SM (a warp still covers 512 bytes of a row).
+    while (p.partial != nullptr && tx > 32 &&
+           (p.n + int64_t(tx) * V - 1) / (int64_t(tx) * V) * partial_rows < int64_t(num_sms(dev)) * 4) {
+        tx >>= 1;
+    }
     p.tx = tx;
     const int64_t gx = (p.n + int64_t(tx) * V - 1) / (int64_t(tx) * V);
     int64_t gy;
@@ -574,21 +613,27 @@ void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaSt
     p.rows_per_block = (p.m + gy - 1) / gy;
     TPB_CHECK(gx < (int64_t(1) << 31), "activation_backward: too many columns");
     const dim3 grid{unsigned(gx), unsigned(gy), 1};
-    if (p.partial != nullptr) launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, ALIGNED, true>, grid, kThreads, 0, s, p);
-    else launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, ALIGNED, false>, grid, kThreads, 0, s, p);
+    if (p.partial != nullptr) launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, MODE, true>, grid, kThreads, 0, s, p);
+    else launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, MODE, false>, grid, kThreads, 0, s, p);
     check_launch("ffn_backward");
 }
 
 template <typename T, bool GATED>
 void dispatch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaStream_t s) {
-    const bool vec = p.n % 8 == 0 && rows16(p.dy, p.sdy_m, sizeof(T)) && rows16(p.z, p.sz_m, sizeof(T)) &&
-                     rows16(p.z, p.sz_p, sizeof(T)) && rows16(p.dz, p.sdz_m, sizeof(T)) &&
-                     rows16(p.dz, p.sdz_p, sizeof(T)) && reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    constexpr size_t es = sizeof(T);
+    const bool aligned = p.n % 8 == 0 && rows16(p.dy, p.sdy_m, es) && rows16(p.z, p.sz_m, es) &&
+                         rows16(p.z, p.sz_p, es) && rows16(p.dz, p.sdz_m, es) && rows16(p.dz, p.sdz_p, es) &&
+                         reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    const bool words = p.n % 2 == 0 && rows4(p.dy, p.sdy_m, es) && rows4(p.z, p.sz_m, es) && rows4(p.z, p.sz_p, es) &&
+                       rows4(p.dz, p.sdz_m, es) && rows4(p.dz, p.sdz_p, es) &&
+                       reinterpret_cast<uintptr_t>(p.values) % 2 == 0;
     if (p.values != nullptr) {
-        if (vec) launch_backward<T, GATED, true, kAligned>(p, partial_rows, dev, s);
+        if (aligned) launch_backward<T, GATED, true, kAligned>(p, partial_rows, dev, s);
+        else if (words) launch_backward<T, GATED, true, kWords>(p, partial_rows, dev, s);
         else launch_backward<T, GATED, true, kAnywhere>(p, partial_rows, dev, s);
     } else {
-        if (vec) launch_backward<T, GATED, false, kAligned>(p, partial_rows, dev, s);
+        if (aligned) launch_backward<T, GATED, false, kAligned>(p, partial_rows, dev, s);
+        else if (words) launch_backward<T, GATED, false, kWords>(p, partial_rows, dev, s);
         else launch_backward<T, GATED, false, kAnywhere>(p, partial_rows, dev, s);
     }
 }
@@ -604,14 +649,16 @@ void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t 
 }
 
 // An operand of a product, copied into `work` (rows of n elements rounded up
-// to 16 bytes) where its rows start off 16-byte boundaries.
+// to 128 bytes) where its rows start off 16-byte boundaries.  Rows that start
+// inside a 32-byte sector cost the tensor-map loads a fifth sector for every
+// four (dx of 1001 x 5460 -> 1000: 37 us on 16-byte boundaries).
 struct Aligned {
     const void* data;
     int64_t pitch;
 };
 Aligned align_rows(const void* src, int64_t pitch, int64_t rows, int64_t n, int es, void* work, const char* what,
                    cudaStream_t s) {
-    const int64_t per = 16 / es, aligned = (n + per - 1) / per * per;
+    const int64_t per = 16 / es, line = 128 / es, aligned = (n + line - 1) / line * line;
     if (aligned16(src) && pitch > 0 && pitch % per == 0) return {src, pitch};
     if (aligned16(src) && rows == 1) return {src, aligned};  // there is no second row
     TPB_CHECK(work != nullptr && aligned16(work), "%s: rows off 16-byte boundaries need an aligned workspace", what);
@@ -805,14 +852,17 @@ int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, con
             p.exponents = static_cast<const uint8_t*>(exponents->data);
             p.n = n;
             p.units = make_units(m, n);
-            const bool vec = rows16(p.y, p.sy_m, sizeof(scalar_t));
-            if (vec && n % 16 == 0 && aligned16(p.values)) {
-                launch_pdl(checkpoint_unpack_kernel<scalar_t, 16, kAligned>, unit_blocks(p.units, 2, 2), kThreads, 0, s, p);
-            } else if (vec && n % 8 == 0 && reinterpret_cast<uintptr_t>(p.values) % 8 == 0) {
-                launch_pdl(checkpoint_unpack_kernel<scalar_t, 8, kAligned>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
-            } else {
-                launch_pdl(checkpoint_unpack_kernel<scalar_t, 8, kAnywhere>, unit_blocks(p.units, 4, 4), kThreads, 0, s, p);
-            }
+            const bool aligned = n % 8 == 0 && rows16(p.y, p.sy_m, sizeof(scalar_t)) &&
+                                 reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+            const bool words = n % 2 == 0 && rows4(p.y, p.sy_m, sizeof(scalar_t)) &&
+                               reinterpret_cast<uintptr_t>(p.values) % 2 == 0;
+            const auto go = [&](auto kernel, int v) {
+                launch_pdl(kernel, unit_blocks(p.units, kCkptBlock / v, 32 / v), kThreads, 0, s, p);
+            };
+            if (aligned && n % 16 == 0 && aligned16(p.values)) go(checkpoint_unpack_kernel<scalar_t, 16, kAligned>, 16);
+            else if (aligned) go(checkpoint_unpack_kernel<scalar_t, 8, kAligned>, 8);
+            else if (words) go(checkpoint_unpack_kernel<scalar_t, 8, kWords>, 8);
+            else go(checkpoint_unpack_kernel<scalar_t, 8, kAnywhere>, 8);
             check_launch("checkpoint_unpack");
         });
     });

@@ -1075,7 +1075,7 @@ def _align_elements(t: torch.Tensor, pitch: int, rows: int, n: int, reads: int) 
         return 0
     if t.dtype == torch.float32 and reads < 4:
         return 0
-    return rows * ((n + per - 1) // per * per)
+    return rows * -(-n // (8 * per)) * 8 * per
 
 
 def _layer_operands(what: str, input, weight, bias, parts: int):
@@ -1250,10 +1250,10 @@ def _layer_backward(what: str, grad_output, input, weight, saved, activation, pa
     db = weight.new_empty((out,)) if want_b else None
     if not (want_x or want_w or want_b):
         return None, None, None
-    # Workspace: dz [rows, out] with rows on 16-byte boundaries, as the two
-    # products read it, the bias gradient's partial sums (fp32), and copies of
+    # Workspace: dz [rows, out] with rows on 128-byte boundaries, as the two
+    # products read it best, the bias gradient's partial sums (fp32), and copies of
     # operands whose rows start elsewhere.
-    per = 16 // input.element_size()
+    per = 128 // input.element_size()
     pitch = (out + per - 1) // per * per
     groups = min(max(rows // 16, 1), 128) if want_b else 0
     dy, sdy = _rows(grad_output, n)
