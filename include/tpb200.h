@@ -461,7 +461,8 @@ typedef struct tpb_layer {
 int tp_b200_layer_forward(const tpb_layer* layer, void* stream);
 
 /* Its gradients: dz (see tp_b200_activation_backward) from dy and what was
- * saved -- either `saved`, contiguous, or values and exponents -- and from it
+ * saved -- either `saved`, contiguous, or values and exponents; neither is
+ * needed or read for parts 1 without an activation -- and from it
  * dx [m, k] = dz w, dw [parts * n, k] = dz^T x (both contiguous), db [parts *
  * n] = the column sums of dz before its rounding.  dx, dw, db may be NULL.
  * dz: workspace [m, parts * n], row stride dz_stride; partial: workspace of

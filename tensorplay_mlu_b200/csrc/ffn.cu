@@ -594,9 +594,9 @@ void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaSt
     int tx = 1;
     while (tx < kThreads && int64_t(tx) * V < p.n) tx <<= 1;
     // Where the partial sums fix the rows' split, narrower blocks until there
-    // are four for every SM (a warp still covers 512 bytes of a row).
+    // are sixteen for every SM (a warp still covers 512 bytes of a row).
     while (p.partial != nullptr && tx > 32 &&
-           (p.n + int64_t(tx) * V - 1) / (int64_t(tx) * V) * partial_rows < int64_t(num_sms(dev)) * 4) {
+           (p.n + int64_t(tx) * V - 1) / (int64_t(tx) * V) * partial_rows < int64_t(num_sms(dev)) * 16) {
         tx >>= 1;
     }
     p.tx = tx;
@@ -974,7 +974,8 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             if (a->db != nullptr && wide > 0) TPB_CUDA(cudaMemsetAsync(a->db, 0, size_t(wide) * es, s));
             return;
         }
-        TPB_CHECK(a->dy != nullptr && a->dz != nullptr && (a->saved != nullptr || a->values != nullptr),
+        const bool linear = a->parts == 1 && a->act == TPB_ACT_NONE;  // dz = dy, whatever z is
+        TPB_CHECK(a->dy != nullptr && a->dz != nullptr && (linear || a->saved != nullptr || a->values != nullptr),
                   "layer_backward: null operand");
         TPB_CHECK(a->dz_stride >= wide, "layer_backward: the workspace's rows hold %lld elements, not %lld",
                   (long long)a->dz_stride, (long long)wide);
@@ -983,15 +984,25 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
         const int dev = device_of(a->dz);
         DeviceGuard guard(dev);
         cudaStream_t s = resolve_stream(stream, dev);
-        TPB_DISPATCH_FFN(a->dtype, "layer_backward", {
+        const void* dz = a->dz;
+        int64_t dz_stride = a->dz_stride;
+        if (linear && a->db == nullptr && (a->dtype == TPB_F32 || (rows16(a->dy, a->dy_stride, es) && a->dy_stride > 0))) {
+            dz = a->dy;  // as it lies
+            dz_stride = a->dy_stride;
+        } else TPB_DISPATCH_FFN(a->dtype, "layer_backward", {
             BackwardParams<scalar_t> p{};
             p.dy = static_cast<const scalar_t*>(a->dy);
             p.sdy_m = a->dy_stride;
-            p.z = static_cast<const scalar_t*>(a->saved);
-            p.sz_m = wide;
-            p.sz_p = n;
-            p.values = static_cast<const int8_t*>(a->values);
-            p.exponents = static_cast<const uint8_t*>(a->exponents);
+            if (linear) {  // any readable rows
+                p.z = p.dy;
+                p.sz_m = p.sdy_m;
+            } else {
+                p.z = static_cast<const scalar_t*>(a->saved);
+                p.sz_m = wide;
+                p.sz_p = n;
+                p.values = static_cast<const int8_t*>(a->values);
+                p.exponents = static_cast<const uint8_t*>(a->exponents);
+            }
             p.nb = (n + kCkptBlock - 1) / kCkptBlock;
             p.dz = static_cast<scalar_t*>(a->dz);
             p.sdz_m = a->dz_stride;
@@ -1028,8 +1039,8 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             q.M = m;
             q.N = k;
             q.K = wide;
-            q.x = a->dz;
-            q.sx_m = a->dz_stride;
+            q.x = dz;
+            q.sx_m = dz_stride;
             q.sx_k = 1;
             q.w = w.data;
             q.sw_n = 1;
@@ -1044,9 +1055,9 @@ int tp_b200_layer_backward(const tpb_layer_grad* a, void* stream) {
             q.M = wide;
             q.N = k;
             q.K = m;
-            q.x = a->dz;
+            q.x = dz;
             q.sx_m = 1;
-            q.sx_k = a->dz_stride;
+            q.sx_k = dz_stride;
             q.w = x.data;
             q.sw_n = 1;
             q.sw_k = x.pitch;

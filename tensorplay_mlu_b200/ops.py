@@ -1238,7 +1238,7 @@ def _layer_backward(what: str, grad_output, input, weight, saved, activation, pa
         values, exponents = saved
         _checkpoint_check(what, values, exponents, wide, input.device)
         values, exponents = _dense(values), _dense(exponents)
-    else:
+    elif saved is not None or parts == 2 or code:
         _ffn_check(what, input, saved)
         if saved is None or tuple(saved.shape) != wide:
             raise RuntimeError(f"{what}: expected saved pre-activations of shape {list(wide)}, got "
@@ -1319,7 +1319,9 @@ def linear_act(input, weight, bias=None, residual=None, activation: str = "none"
 def native_linear_act_backward(grad_output, input, weight, saved, activation: str = "none",
                                output_mask=(True, True, True)):
     """(dinput, dweight, dbias) of :func:`native_linear_act`, each None where
-    ``output_mask`` says so; the residual's gradient is ``grad_output``."""
+    ``output_mask`` says so; the residual's gradient is ``grad_output``.
+    ``saved`` is what the forward pass returned; without an activation it is
+    not read and may be None."""
     return _layer_backward("native_linear_act_backward", grad_output, input, weight, saved, activation, 1,
                            output_mask)
 

@@ -248,6 +248,26 @@ def test_backward_output_mask(ops):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [40, 41])
+def test_backward_without_an_activation_needs_nothing_saved(ops, dtype, n):
+    """dz is dy, read where it lies (rows on 16-byte boundaries) or copied; a
+    saved tensor changes nothing."""
+    m, k = 70, 136
+    x, w = dev(rand(m, k, dtype=dtype, seed=1)), dev(rand(n, k, dtype=dtype, seed=2))
+    wide = dev(rand(m, n + 8, dtype=dtype, seed=3))
+    nan = torch.full((m, n), math.nan, dtype=dtype, device="cuda")
+    for dy in (wide[:, :n].contiguous(), wide[:, :n], wide[:, 5:5 + n], wide[:1, :n].expand(m, n)):
+        for mask in ((True, True, True), (True, True, False)):
+            a = ops.native_linear_act_backward(dy, x, w, None, "none", mask)
+            b = ops.native_linear_act_backward(dy, x, w, nan, "none", mask)
+            c = ops.native_linear_act_backward(dy.contiguous(), x, w, nan, "none", (True, True, True))
+            for i in range(3):
+                assert (a[i] is None) == (not mask[i])
+                if mask[i]:
+                    assert torch.equal(a[i], b[i]) and torch.equal(a[i], c[i])
+
+
 def test_gradients_against_differences(ops):
     """The backward passes against central differences of the forward ones, in
     float32: with a step of 2^-6 the difference quotient of a loss of M N terms
@@ -549,7 +569,8 @@ def test_refusals(ops):
         (lambda: ops.linear_act(x, w.view(2, 4, 16)), "2-d weight"),
         (lambda: ops.native_linear_act_backward(x, x, w, x), "gradient of shape"),
         (lambda: ops.native_linear_act_backward(dev(rand(4, 8)), x, w, x), "pre-activations of shape"),
-        (lambda: ops.native_linear_act_backward(dev(rand(4, 8)), x, w, None), "pre-activations of shape"),
+        (lambda: ops.native_linear_act_backward(dev(rand(4, 8)), x, w, None, "relu"), "pre-activations of shape"),
+        (lambda: ops.native_gated_linear_backward(dev(rand(4, 4)), x, w, None, "none"), "pre-activations of shape"),
         (lambda: ops.native_linear_act_backward(dev(rand(4, 8)), x, w, (x,)), "values, exponents"),
         (lambda: ops.native_linear_act_backward(dev(rand(4, 8)), x, w, (x, x)), "int8 values"),
         (lambda: ops.checkpoint_pack(x.int()), "bfloat16, float16 or float32"),
