@@ -590,11 +590,13 @@ void launch_forward(ForwardParams<T>& p, cudaStream_t s) {
 template <typename T, bool GATED, bool SAVED8, int MODE>
 void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaStream_t s) {
     constexpr int V = 8;
-    // Threads along the columns: enough for one row, at most the block.
+    // Threads along the columns: enough for one row, at most the block, or two
+    // warps where the rows' split is free (a warp covers 512 bytes of a row).
+    const int widest = p.partial != nullptr ? kThreads : 64;
     int tx = 1;
-    while (tx < kThreads && int64_t(tx) * V < p.n) tx <<= 1;
+    while (tx < widest && int64_t(tx) * V < p.n) tx <<= 1;
     // Where the partial sums fix the rows' split, narrower blocks until there
-    // are sixteen for every SM (a warp still covers 512 bytes of a row).
+    // are sixteen for every SM.
     while (p.partial != nullptr && tx > 32 &&
            (p.n + int64_t(tx) * V - 1) / (int64_t(tx) * V) * partial_rows < int64_t(num_sms(dev)) * 16) {
         tx >>= 1;
@@ -605,9 +607,9 @@ void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaSt
     if (p.partial != nullptr) {
         gy = partial_rows;
     } else {
-        // About eight blocks an SM, and no more than one pass of rows needs.
+        // About 32 blocks an SM, and no more than one pass of rows needs.
         const int64_t pass = int64_t(kThreads / tx) * rows_at_once<T, GATED>();
-        gy = std::max<int64_t>(1, std::min<int64_t>((p.m + pass - 1) / pass, (int64_t(num_sms(dev)) * 8 + gx - 1) / gx));
+        gy = std::max<int64_t>(1, std::min<int64_t>((p.m + pass - 1) / pass, (int64_t(num_sms(dev)) * 32 + gx - 1) / gx));
         gy = std::min<int64_t>(gy, 65535);
     }
     p.rows_per_block = (p.m + gy - 1) / gy;
