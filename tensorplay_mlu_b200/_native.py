@@ -60,7 +60,9 @@ class TpbTensor(ctypes.Structure):
 
 
 def describe(t: torch.Tensor) -> TpbTensor:
-    """Descriptor of a strided tensor (device or host memory)."""
+    """Descriptor of a strided tensor (device or host memory).  It keeps the
+    tensor: a temporary described in a call's arguments would otherwise give
+    its memory to the next temporary before the call is made."""
     if t.dim() > MAX_DIMS:
         raise RuntimeError(f"at most {MAX_DIMS} dimensions are supported, got {t.dim()}")
     try:
@@ -68,6 +70,7 @@ def describe(t: torch.Tensor) -> TpbTensor:
     except KeyError as error:
         raise TypeError(f"dtype {t.dtype} is not supported by the B200 backend") from error
     d = TpbTensor()
+    d.keep = t
     d.data = t.data_ptr() if t.numel() else None
     d.dtype = code
     d.ndim = t.dim()
