@@ -460,8 +460,8 @@ typedef struct tpb_layer {
 } tpb_layer;
 int tp_b200_layer_forward(const tpb_layer* layer, void* stream);
 
-/* Its gradients: dz (see tp_b200_activation_backward) from dy and what was
- * saved -- either `saved`, contiguous, or values and exponents; neither is
+/* Its gradients: dz = dy act'(z), or [dy zu act'(zg) | dy act(zg)] for the
+ * gated block, from dy and what was saved -- either `saved`, contiguous, or values and exponents; neither is
  * needed or read for parts 1 without an activation -- and from it
  * dx [m, k] = dz w, dw [parts * n, k] = dz^T x (both contiguous), db [parts *
  * n] = the column sums of dz before its rounding.  dx, dw, db may be NULL.
@@ -491,23 +491,25 @@ typedef struct tpb_layer_grad {
 } tpb_layer_grad;
 int tp_b200_layer_backward(const tpb_layer_grad* grad, void* stream);
 
-/* y = act(z) [+ residual] for z [rows, n], y = act(z0) * z1 [+ residual] for
- * z [rows, 2, n]; y [rows, n] may be NULL.  values / exponents (may be NULL)
- * receive the checkpoint of z.  Rows may be strided; computed in fp32 and
- * rounded once. */
-int tp_b200_activation_forward(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
-                               const tpb_tensor* z, const tpb_tensor* residual, int act, void* stream);
-/* The gradient of activation_forward's z (shaped like dz): dz = dy * act'(z),
- * or dz0 = dy * z1 * act'(z0) and dz1 = dy * act(z0).  z is a tensor, or NULL
- * and given as a checkpoint.  partial (may be NULL): fp32 [b, parts * n],
- * 1 <= b <= 65535, receives the column sums of dz over b groups of rows,
- * taken before dz is rounded (their sum is the bias gradient). */
-int tp_b200_activation_backward(const tpb_tensor* dz, const tpb_tensor* partial, const tpb_tensor* dy,
-                                const tpb_tensor* z, const tpb_tensor* values, const tpb_tensor* exponents, int act,
-                                void* stream);
-/* y [rows, n] = what a checkpoint stands for, rounded to y's dtype. */
-int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
-                              void* stream);
+/* 8-bit checkpoints of rows of n elements (see above).
+ *   pack      x -> values, exponents
+ *   unpack    values, exponents -> y, rounded to dtype
+ *   backward  y = x * act'(z), x the gradient and z the checkpoint
+ * Rows of x and y may be strided (elements); values [rows, n] and exponents
+ * [rows, ceil(n / 32)] are contiguous. */
+typedef struct tpb_checkpoint {
+    int32_t dtype, act;
+    int64_t rows, n;
+    const void* x;
+    int64_t x_stride;
+    void* y;
+    int64_t y_stride;
+    void* values;
+    void* exponents;
+} tpb_checkpoint;
+int tp_b200_checkpoint_pack(const tpb_checkpoint* args, void* stream);
+int tp_b200_checkpoint_unpack(const tpb_checkpoint* args, void* stream);
+int tp_b200_checkpoint_backward(const tpb_checkpoint* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * Collectives over NCCL (replaces tensorplay_mlu/csrc/Cncl.cpp:71-387; same

@@ -80,16 +80,10 @@ def describe(t: torch.Tensor) -> TpbTensor:
     return d
 
 
-# tpb_tensor, tpb_layer and tpb_layer_grad as packed bytes.
-_TENSOR = struct.Struct("Pii16q")
+# tpb_layer, tpb_layer_grad and tpb_checkpoint as packed bytes.
 LAYER = struct.Struct("4i3qPqPqPPqPqPPPPP")
 LAYER_GRAD = struct.Struct("4i4qPqPqPqPPPPPPPqPPP")
-
-
-def describe_rows(t: torch.Tensor, rows: int, n: int, pitch: int) -> TpbTensor:
-    """Descriptor of ``t``'s memory seen as [rows, n] with row stride ``pitch``."""
-    return TpbTensor.from_buffer_copy(_TENSOR.pack(t.data_ptr(), DTYPE_CODES[t.dtype], 2, rows, n, 0, 0, 0, 0, 0, 0,
-                                                   pitch, 1, 0, 0, 0, 0, 0, 0))
+CHECKPOINT = struct.Struct("2i2qPqPqPP")
 
 
 _LOCK = threading.Lock()
@@ -161,9 +155,9 @@ _SIGNATURES = {
     "tp_b200_masked_scale": ([_T, _T, _T, _D, _P], _I),
     "tp_b200_layer_forward": ([_P, _P], _I),
     "tp_b200_layer_backward": ([_P, _P], _I),
-    "tp_b200_activation_forward": ([_T, _T, _T, _T, _T, _I, _P], _I),
-    "tp_b200_activation_backward": ([_T, _T, _T, _T, _T, _T, _I, _P], _I),
-    "tp_b200_checkpoint_unpack": ([_T, _T, _T, _P], _I),
+    "tp_b200_checkpoint_pack": ([_P, _P], _I),
+    "tp_b200_checkpoint_unpack": ([_P, _P], _I),
+    "tp_b200_checkpoint_backward": ([_P, _P], _I),
     "tp_b200_nccl_last_error": ([], ctypes.c_char_p),
     "tp_b200_nccl_unique_id_bytes": ([], _I),
     "tp_b200_nccl_get_unique_id": ([_P], _I),

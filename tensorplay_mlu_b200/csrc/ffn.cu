@@ -502,48 +502,8 @@ __global__ void __launch_bounds__(kThreads) column_sum_kernel(const float* __res
     }
 }
 
-void require_dtype(const tpb_tensor& t, int dtype, const char* what) {
-    TPB_CHECK(t.dtype == dtype, "%s: expected %s, got %s", what, dtype_name(dtype), dtype_name(t.dtype));
-}
-
 void require_act(int act, const char* what) {
     TPB_CHECK(act >= TPB_ACT_NONE && act <= TPB_ACT_SILU, "%s: unknown activation %d", what, act);
-}
-
-void require_float(const tpb_tensor& t, const char* what) {
-    TPB_CHECK(t.dtype == TPB_BF16 || t.dtype == TPB_F16 || t.dtype == TPB_F32,
-              "%s: expected bfloat16, float16 or float32, got %s", what, dtype_name(t.dtype));
-}
-
-// [rows, n] or [rows, 2, n] with unit stride along n.
-void require_rows(const tpb_tensor& t, const char* what) {
-    TPB_CHECK(t.ndim == 2 || (t.ndim == 3 && t.sizes[1] == 2), "%s: expected [rows, n] or [rows, 2, n]", what);
-    TPB_CHECK(t.strides[t.ndim - 1] == 1 || t.sizes[t.ndim - 1] <= 1, "%s: needs unit stride along its last dimension",
-              what);
-}
-
-void require_same(const tpb_tensor& a, const tpb_tensor& b, const char* what) {
-    TPB_CHECK(a.ndim == b.ndim, "%s: rank mismatch (%d vs %d)", what, a.ndim, b.ndim);
-    for (int i = 0; i < a.ndim; ++i) {
-        TPB_CHECK(a.sizes[i] == b.sizes[i], "%s: size mismatch at dimension %d (%lld vs %lld)", what, i,
-                  (long long)a.sizes[i], (long long)b.sizes[i]);
-    }
-}
-
-// int8 values shaped like `z` and uint8 exponents [.., ceil(n / 32)], dense.
-void require_checkpoint(const tpb_tensor* values, const tpb_tensor* exponents, const tpb_tensor& z, const char* what) {
-    check_tensor(values, what);
-    check_tensor(exponents, what);
-    require_dtype(*values, TPB_I8, what);
-    require_dtype(*exponents, TPB_U8, what);
-    require_same(*values, z, what);
-    TPB_CHECK(is_contiguous(*values) && is_contiguous(*exponents), "%s: checkpoints are contiguous", what);
-    TPB_CHECK(exponents->ndim == z.ndim, "%s: exponents need the values' rank", what);
-    for (int i = 0; i < z.ndim; ++i) {
-        const int64_t want = i == z.ndim - 1 ? (z.sizes[i] + kCkptBlock - 1) / kCkptBlock : z.sizes[i];
-        TPB_CHECK(exponents->sizes[i] == want, "%s: exponents have %lld, not %lld, at dimension %d", what,
-                  (long long)exponents->sizes[i], (long long)want, i);
-    }
 }
 
 // Rows on 4-byte boundaries (checkpoint values of even rows: 2-byte ones).
@@ -613,7 +573,7 @@ void launch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cudaSt
         gy = std::min<int64_t>(gy, 65535);
     }
     p.rows_per_block = (p.m + gy - 1) / gy;
-    TPB_CHECK(gx < (int64_t(1) << 31), "activation_backward: too many columns");
+    TPB_CHECK(gx < (int64_t(1) << 31), "feed-forward gradients: too many columns");
     const dim3 grid{unsigned(gx), unsigned(gy), 1};
     if (p.partial != nullptr) launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, MODE, true>, grid, kThreads, 0, s, p);
     else launch_pdl(ffn_backward_kernel<T, V, GATED, SAVED8, MODE, false>, grid, kThreads, 0, s, p);
@@ -640,6 +600,28 @@ void dispatch_backward(BackwardParams<T>& p, int64_t partial_rows, int dev, cuda
     }
 }
 
+#define TPB_DISPATCH_FFN(dtype, what, ...)                                        \
+    switch (dtype) {                                                              \
+        case TPB_F16: { using scalar_t = __half; __VA_ARGS__; break; }            \
+        case TPB_F32: { using scalar_t = float; __VA_ARGS__; break; }             \
+        case TPB_BF16: { using scalar_t = __nv_bfloat16; __VA_ARGS__; break; }    \
+        default: TPB_CHECK(false, "%s: unsupported dtype %s", what, dtype_name(dtype)); \
+    }
+
+template <typename T>
+void launch_unpack(const UnpackParams<T>& p, cudaStream_t s) {
+    const bool aligned = p.n % 8 == 0 && rows16(p.y, p.sy_m, sizeof(T)) && reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
+    const bool words = p.n % 2 == 0 && rows4(p.y, p.sy_m, sizeof(T)) && reinterpret_cast<uintptr_t>(p.values) % 2 == 0;
+    const auto go = [&](auto kernel, int v) {
+        launch_pdl(kernel, unit_blocks(p.units, kCkptBlock / v, 32 / v), kThreads, 0, s, p);
+    };
+    if (aligned && p.n % 16 == 0 && aligned16(p.values)) go(checkpoint_unpack_kernel<T, 16, kAligned>, 16);
+    else if (aligned) go(checkpoint_unpack_kernel<T, 8, kAligned>, 8);
+    else if (words) go(checkpoint_unpack_kernel<T, 8, kWords>, 8);
+    else go(checkpoint_unpack_kernel<T, 8, kAnywhere>, 8);
+    check_launch("checkpoint_unpack");
+}
+
 void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t k, const char* what) {
     TPB_CHECK(dtype == TPB_BF16 || dtype == TPB_F16 || dtype == TPB_F32,
               "%s: expected bfloat16, float16 or float32, got %s", what, dtype_name(dtype));
@@ -648,6 +630,25 @@ void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t 
     const int64_t limit = int64_t(1) << 30;
     TPB_CHECK(m >= 0 && n >= 0 && k >= 0 && m < limit && n < limit && k < limit,
               "%s: sizes %lld, %lld, %lld out of range", what, (long long)m, (long long)n, (long long)k);
+}
+
+// A checkpoint entry point: its checks, then body(T{}, device, stream).
+template <typename F>
+int checkpoint_call(const tpb_checkpoint* a, const char* what, bool reads, bool writes, void* stream, F&& body) {
+    return guarded([&] {
+        TPB_CHECK(a != nullptr, "%s: null arguments", what);
+        require_layer(a->dtype, a->act, 1, 0, 0, 0, what);
+        TPB_CHECK(a->rows >= 0 && a->n >= 0 && a->n < (int64_t(1) << 40) && a->rows < (int64_t(1) << 40),
+                  "%s: sizes %lld, %lld out of range", what, (long long)a->rows, (long long)a->n);
+        if (a->rows == 0 || a->n == 0) return;
+        TPB_CHECK(a->values != nullptr && a->exponents != nullptr && (!reads || a->x != nullptr) &&
+                      (!writes || a->y != nullptr),
+                  "%s: null operand", what);
+        const int dev = device_of(a->values);
+        DeviceGuard guard(dev);
+        cudaStream_t s = resolve_stream(stream, dev);
+        TPB_DISPATCH_FFN(a->dtype, what, body(scalar_t(0.0f), dev, s));
+    });
 }
 
 // An operand of a product, copied into `work` (rows of n elements rounded up
@@ -704,14 +705,6 @@ void run_gemm(const GemmProblem& p, int dev, cudaStream_t s) {
     if (!gemm_tc(p, dev, s)) gemm_simt(p, dev, s);
 }
 
-#define TPB_DISPATCH_FFN(dtype, what, ...)                                        \
-    switch (dtype) {                                                              \
-        case TPB_F16: { using scalar_t = __half; __VA_ARGS__; break; }            \
-        case TPB_F32: { using scalar_t = float; __VA_ARGS__; break; }             \
-        case TPB_BF16: { using scalar_t = __nv_bfloat16; __VA_ARGS__; break; }    \
-        default: TPB_CHECK(false, "%s: unsupported dtype %s", what, dtype_name(dtype)); \
-    }
-
 }  // namespace
 }  // namespace tpb
 
@@ -719,154 +712,49 @@ using namespace tpb;
 
 extern "C" {
 
-int tp_b200_activation_forward(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
-                               const tpb_tensor* z, const tpb_tensor* residual, int act, void* stream) {
-    return guarded([&] {
-        check_tensor(z, "activation_forward z");
-        require_float(*z, "activation_forward z");
-        require_rows(*z, "activation_forward z");
-        require_act(act, "activation_forward");
-        const bool gated = z->ndim == 3;
-        const int64_t m = z->sizes[0], n = z->sizes[z->ndim - 1];
-        for (const tpb_tensor* t : {y, residual}) {
-            if (t == nullptr) continue;
-            check_tensor(t, "activation_forward result or residual");
-            require_dtype(*t, z->dtype, "activation_forward result or residual");
-            require_rows(*t, "activation_forward result or residual");
-            TPB_CHECK(t->ndim == 2 && t->sizes[0] == m && t->sizes[1] == n,
-                      "activation_forward: result and residual are [%lld, %lld]", (long long)m, (long long)n);
-        }
-        TPB_CHECK((values == nullptr) == (exponents == nullptr), "activation_forward: a checkpoint is values and exponents");
-        TPB_CHECK(y != nullptr || values != nullptr, "activation_forward: nothing to compute");
-        if (values != nullptr) require_checkpoint(values, exponents, *z, "activation_forward checkpoint");
-        if (m == 0 || n == 0) return;
-        const int dev = device_of(z->data);
-        DeviceGuard guard(dev);
-        cudaStream_t s = resolve_stream(stream, dev);
-        TPB_DISPATCH_FFN(z->dtype, "activation_forward", {
-            ForwardParams<scalar_t> p{};
-            p.z = static_cast<const scalar_t*>(z->data);
-            p.sz_m = z->strides[0];
-            p.sz_p = gated ? z->strides[1] : 0;
-            if (residual != nullptr) {
-                p.residual = static_cast<const scalar_t*>(residual->data);
-                p.sr_m = residual->strides[0];
-            }
-            if (y != nullptr) {
-                p.y = static_cast<scalar_t*>(y->data);
-                p.sy_m = y->strides[0];
-            }
-            if (values != nullptr) {
-                p.values = static_cast<int8_t*>(values->data);
-                p.exponents = static_cast<uint8_t*>(exponents->data);
-            }
-            p.n = n;
-            p.act = act;
-            p.units = make_units(m, n);
-            if (gated) launch_forward<scalar_t, true>(p, s);
-            else launch_forward<scalar_t, false>(p, s);
-        });
+int tp_b200_checkpoint_pack(const tpb_checkpoint* a, void* stream) {
+    return checkpoint_call(a, "checkpoint_pack", true, false, stream, [&](auto zero, int, cudaStream_t s) {
+        using T = decltype(zero);
+        ForwardParams<T> p{};
+        p.z = static_cast<const T*>(a->x);
+        p.sz_m = a->x_stride;
+        p.values = static_cast<int8_t*>(a->values);
+        p.exponents = static_cast<uint8_t*>(a->exponents);
+        p.n = a->n;
+        p.units = make_units(a->rows, a->n);
+        launch_forward<T, false>(p, s);
     });
 }
 
-int tp_b200_activation_backward(const tpb_tensor* dz, const tpb_tensor* partial, const tpb_tensor* dy,
-                                const tpb_tensor* z, const tpb_tensor* values, const tpb_tensor* exponents, int act,
-                                void* stream) {
-    return guarded([&] {
-        check_tensor(dz, "activation_backward dz");
-        check_tensor(dy, "activation_backward dy");
-        require_float(*dz, "activation_backward dz");
-        require_dtype(*dy, dz->dtype, "activation_backward dy");
-        require_rows(*dz, "activation_backward dz");
-        require_rows(*dy, "activation_backward dy");
-        require_act(act, "activation_backward");
-        const bool gated = dz->ndim == 3;
-        const int64_t m = dz->sizes[0], n = dz->sizes[dz->ndim - 1];
-        TPB_CHECK(dy->ndim == 2 && dy->sizes[0] == m && dy->sizes[1] == n, "activation_backward: dy is [%lld, %lld]",
-                  (long long)m, (long long)n);
-        TPB_CHECK((z == nullptr) != (values == nullptr),
-                  "activation_backward: the activation's input is given as a tensor or as a checkpoint");
-        if (z != nullptr) {
-            check_tensor(z, "activation_backward z");
-            require_dtype(*z, dz->dtype, "activation_backward z");
-            require_rows(*z, "activation_backward z");
-            require_same(*z, *dz, "activation_backward z");
-        } else {
-            require_checkpoint(values, exponents, *dz, "activation_backward checkpoint");
-        }
-        int64_t partial_rows = 0;
-        if (partial != nullptr) {
-            check_tensor(partial, "activation_backward partial");
-            require_dtype(*partial, TPB_F32, "activation_backward partial");
-            partial_rows = partial->sizes[0];
-            TPB_CHECK(partial->ndim == 2 && is_contiguous(*partial) && partial_rows >= 1 && partial_rows <= 65535 &&
-                          partial->sizes[1] == (gated ? 2 : 1) * n,
-                      "activation_backward: partial sums are [1 .. 65535, parts * n], contiguous");
-        }
-        if (n == 0 || (m == 0 && partial == nullptr)) return;
-        const int dev = device_of(partial != nullptr ? partial->data : dz->data);
-        DeviceGuard guard(dev);
-        cudaStream_t s = resolve_stream(stream, dev);
-        TPB_DISPATCH_FFN(dz->dtype, "activation_backward", {
-            BackwardParams<scalar_t> p{};
-            p.dy = static_cast<const scalar_t*>(dy->data);
-            p.sdy_m = dy->strides[0];
-            if (z != nullptr) {
-                p.z = static_cast<const scalar_t*>(z->data);
-                p.sz_m = z->strides[0];
-                p.sz_p = gated ? z->strides[1] : 0;
-            } else {
-                p.values = static_cast<const int8_t*>(values->data);
-                p.exponents = static_cast<const uint8_t*>(exponents->data);
-                p.nb = (n + kCkptBlock - 1) / kCkptBlock;
-            }
-            p.dz = static_cast<scalar_t*>(dz->data);
-            p.sdz_m = dz->strides[0];
-            p.sdz_p = gated ? dz->strides[1] : 0;
-            if (partial != nullptr) p.partial = static_cast<float*>(partial->data);
-            p.m = m;
-            p.n = n;
-            p.act = act;
-            if (gated) dispatch_backward<scalar_t, true>(p, partial_rows, dev, s);
-            else dispatch_backward<scalar_t, false>(p, partial_rows, dev, s);
-        });
+int tp_b200_checkpoint_unpack(const tpb_checkpoint* a, void* stream) {
+    return checkpoint_call(a, "checkpoint_unpack", false, true, stream, [&](auto zero, int, cudaStream_t s) {
+        using T = decltype(zero);
+        UnpackParams<T> p{};
+        p.y = static_cast<T*>(a->y);
+        p.sy_m = a->y_stride;
+        p.values = static_cast<const int8_t*>(a->values);
+        p.exponents = static_cast<const uint8_t*>(a->exponents);
+        p.n = a->n;
+        p.units = make_units(a->rows, a->n);
+        launch_unpack<T>(p, s);
     });
 }
 
-int tp_b200_checkpoint_unpack(const tpb_tensor* y, const tpb_tensor* values, const tpb_tensor* exponents,
-                              void* stream) {
-    return guarded([&] {
-        check_tensor(y, "checkpoint_unpack y");
-        require_float(*y, "checkpoint_unpack y");
-        TPB_CHECK(y->ndim == 2, "checkpoint_unpack: the result is [rows, n]");
-        require_rows(*y, "checkpoint_unpack y");
-        require_checkpoint(values, exponents, *y, "checkpoint_unpack");
-        const int64_t m = y->sizes[0], n = y->sizes[1];
-        if (m == 0 || n == 0) return;
-        const int dev = device_of(y->data);
-        DeviceGuard guard(dev);
-        cudaStream_t s = resolve_stream(stream, dev);
-        TPB_DISPATCH_FFN(y->dtype, "checkpoint_unpack", {
-            UnpackParams<scalar_t> p{};
-            p.y = static_cast<scalar_t*>(y->data);
-            p.sy_m = y->strides[0];
-            p.values = static_cast<const int8_t*>(values->data);
-            p.exponents = static_cast<const uint8_t*>(exponents->data);
-            p.n = n;
-            p.units = make_units(m, n);
-            const bool aligned = n % 8 == 0 && rows16(p.y, p.sy_m, sizeof(scalar_t)) &&
-                                 reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
-            const bool words = n % 2 == 0 && rows4(p.y, p.sy_m, sizeof(scalar_t)) &&
-                               reinterpret_cast<uintptr_t>(p.values) % 2 == 0;
-            const auto go = [&](auto kernel, int v) {
-                launch_pdl(kernel, unit_blocks(p.units, kCkptBlock / v, 32 / v), kThreads, 0, s, p);
-            };
-            if (aligned && n % 16 == 0 && aligned16(p.values)) go(checkpoint_unpack_kernel<scalar_t, 16, kAligned>, 16);
-            else if (aligned) go(checkpoint_unpack_kernel<scalar_t, 8, kAligned>, 8);
-            else if (words) go(checkpoint_unpack_kernel<scalar_t, 8, kWords>, 8);
-            else go(checkpoint_unpack_kernel<scalar_t, 8, kAnywhere>, 8);
-            check_launch("checkpoint_unpack");
-        });
+int tp_b200_checkpoint_backward(const tpb_checkpoint* a, void* stream) {
+    return checkpoint_call(a, "checkpoint_backward", true, true, stream, [&](auto zero, int dev, cudaStream_t s) {
+        using T = decltype(zero);
+        BackwardParams<T> p{};
+        p.dy = static_cast<const T*>(a->x);
+        p.sdy_m = a->x_stride;
+        p.values = static_cast<const int8_t*>(a->values);
+        p.exponents = static_cast<const uint8_t*>(a->exponents);
+        p.nb = (a->n + kCkptBlock - 1) / kCkptBlock;
+        p.dz = static_cast<T*>(a->y);
+        p.sdz_m = a->y_stride;
+        p.m = a->rows;
+        p.n = a->n;
+        p.act = a->act;
+        dispatch_backward<T, false>(p, 0, dev, s);
     });
 }
 

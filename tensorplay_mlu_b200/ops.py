@@ -1101,7 +1101,8 @@ def _checkpoint_empty(like, shape):
 
 
 def _checkpoint_check(what: str, values, exponents, shape, device) -> None:
-    _require_device(values, exponents)
+    if not (_is_device(values) and _is_device(exponents)):
+        _require_device(values, exponents)
     if values.dtype != torch.int8 or exponents.dtype != torch.uint8:
         raise RuntimeError(f"{what}: a checkpoint is int8 values and uint8 exponents, got {values.dtype} and "
                            f"{exponents.dtype}")
@@ -1125,16 +1126,15 @@ def checkpoint_pack(x):
     _ffn_check("checkpoint_pack", x)
     if x.dim() == 0:
         raise RuntimeError("checkpoint_pack: expected at least one dimension")
-    values, exponents = _checkpoint_empty(x, tuple(x.shape))
+    shape = tuple(x.shape)
+    values, exponents = _checkpoint_empty(x, shape)
     numel = x.numel()
     if numel:
-        n = x.shape[-1]
-        rows = numel // n
-        blocks = (n + _BLOCK - 1) // _BLOCK
+        n = shape[-1]
         x, pitch = _rows(x, n)
-        N.check(_lib().tp_b200_activation_forward(
-            None, N.describe_rows(values, rows, n, n), N.describe_rows(exponents, rows, blocks, blocks),
-            N.describe_rows(x, rows, n, pitch), None, 0, _stream(x)), "checkpoint_pack")
+        args = N.CHECKPOINT.pack(N.DTYPE_CODES[x.dtype], 0, numel // n, n, x.data_ptr(), pitch, 0, 0, values.data_ptr(),
+                                 exponents.data_ptr())
+        N.check(_lib().tp_b200_checkpoint_pack(args, _stream(x)), "checkpoint_pack")
     return values, exponents
 
 
@@ -1151,12 +1151,10 @@ def checkpoint_unpack(values, exponents, dtype: torch.dtype):
     numel = out.numel()
     if numel:
         n = values.shape[-1]
-        rows = numel // n
-        blocks = (n + _BLOCK - 1) // _BLOCK
         values, exponents = _dense(values), _dense(exponents)
-        N.check(_lib().tp_b200_checkpoint_unpack(
-            N.describe_rows(out, rows, n, n), N.describe_rows(values, rows, n, n),
-            N.describe_rows(exponents, rows, blocks, blocks), _stream(values)), "checkpoint_unpack")
+        args = N.CHECKPOINT.pack(N.DTYPE_CODES[dtype], 0, numel // n, n, 0, 0, out.data_ptr(), n, values.data_ptr(),
+                                 exponents.data_ptr())
+        N.check(_lib().tp_b200_checkpoint_unpack(args, _stream(values)), "checkpoint_unpack")
     return out
 
 
@@ -1171,15 +1169,12 @@ def checkpoint_activation_backward(grad_output, values, exponents, activation: s
     out = grad_output.new_empty(grad_output.shape)
     numel = out.numel()
     if numel:
-        n = out.shape[-1]
-        rows = numel // n
-        blocks = (n + _BLOCK - 1) // _BLOCK
+        n = grad_output.shape[-1]
         dy, pitch = _rows(grad_output, n)
         values, exponents = _dense(values), _dense(exponents)
-        N.check(_lib().tp_b200_activation_backward(
-            N.describe_rows(out, rows, n, n), None, N.describe_rows(dy, rows, n, pitch), None,
-            N.describe_rows(values, rows, n, n), N.describe_rows(exponents, rows, blocks, blocks), code, _stream(dy)),
-            what)
+        args = N.CHECKPOINT.pack(N.DTYPE_CODES[dy.dtype], code, numel // n, n, dy.data_ptr(), pitch, out.data_ptr(), n,
+                                 values.data_ptr(), exponents.data_ptr())
+        N.check(_lib().tp_b200_checkpoint_backward(args, _stream(dy)), what)
     return out
 
 

@@ -5,10 +5,8 @@ launched here; the pointers are never read."""
 
 from __future__ import annotations
 
-import ctypes
 import os
 import re
-import struct
 import subprocess
 
 import pytest
@@ -61,9 +59,9 @@ def test_null_arguments_are_refused():
     lib = N.lib()
     assert lib.tp_b200_layer_forward(None, None) < 0
     assert lib.tp_b200_layer_backward(None, None) < 0
-    assert lib.tp_b200_activation_forward(None, None, None, None, None, 0, None) < 0
-    assert lib.tp_b200_activation_backward(None, None, None, None, None, None, 0, None) < 0
-    assert lib.tp_b200_checkpoint_unpack(None, None, None, None) < 0
+    assert lib.tp_b200_checkpoint_pack(None, None) < 0
+    assert lib.tp_b200_checkpoint_unpack(None, None) < 0
+    assert lib.tp_b200_checkpoint_backward(None, None) < 0
 
 
 def test_empty_calls_touch_no_device():
@@ -74,53 +72,36 @@ def test_empty_calls_touch_no_device():
     assert lib.tp_b200_layer_backward(N.LAYER_GRAD.pack(*empty.values()), None) == 0
 
 
-def descriptor(shape, dtype=torch.bfloat16, strides=None):
-    t = torch.empty(shape, dtype=dtype)
-    d = N.describe(t)
-    d.data = P
-    for i, s in enumerate(strides or ()):
-        d.strides[i] = s
-    return d
+CHECKPOINT = dict(dtype=BF16, act=2, rows=4, n=40, x=P, x_stride=40, y=P, y_stride=40, values=P, exponents=P)
 
 
-@pytest.mark.parametrize("call,match", [
-    (lambda f: f(descriptor((4, 8)), None, None, descriptor((4, 9)), None, 0, None), "result and residual are"),
-    (lambda f: f(descriptor((4, 8)), None, None, descriptor((4, 8), strides=(16, 2)), None, 0, None), "unit stride"),
-    (lambda f: f(descriptor((4, 8)), None, None, descriptor((4, 3, 8)), None, 0, None), "[rows, 2, n]"),
-    (lambda f: f(descriptor((4, 8)), None, None, descriptor((4, 8), torch.float64), None, 0, None), "float64"),
-    (lambda f: f(descriptor((4, 8), torch.float16), None, None, descriptor((4, 8)), None, 0, None), "expected bfloat16"),
-    (lambda f: f(None, None, None, descriptor((4, 8)), None, 0, None), "nothing to compute"),
-    (lambda f: f(None, descriptor((4, 8), torch.int8), None, descriptor((4, 8)), None, 0, None), "values and exponents"),
-    (lambda f: f(None, descriptor((4, 8), torch.int8), descriptor((4, 2), torch.uint8), descriptor((4, 8)), None, 0, None),
-     "at dimension 1"),
-    (lambda f: f(None, descriptor((4, 8), torch.uint8), descriptor((4, 1), torch.uint8), descriptor((4, 8)), None, 0, None),
-     "expected int8"),
-    (lambda f: f(descriptor((4, 8)), None, None, descriptor((4, 8)), None, 7, None), "unknown activation"),
+@pytest.mark.parametrize("entry", ["pack", "unpack", "backward"])
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=F64), "float64"), (dict(act=8), "unknown activation"), (dict(rows=-1), "out of range"), (dict(n=-3), "out of range"),
+    (dict(n=1 << 50), "out of range"), (dict(values=0), "null operand"), (dict(exponents=0), "null operand"),
 ])
-def test_activation_forward_refusals(call, match):
-    assert call(N.lib().tp_b200_activation_forward) < 0
-    assert match in N.lib().tp_b200_last_error().decode()
+def test_checkpoint_refusals(entry, change, match):
+    assert match in refused(f"tp_b200_checkpoint_{entry}", N.CHECKPOINT, CHECKPOINT, **change)
 
 
-@pytest.mark.parametrize("call,match", [
-    (lambda f: f(descriptor((4, 8)), None, descriptor((4, 8)), None, None, None, 0, None), "as a tensor or as a checkpoint"),
-    (lambda f: f(descriptor((4, 8)), None, descriptor((4, 7)), descriptor((4, 8)), None, None, 0, None), "dy is"),
-    (lambda f: f(descriptor((4, 8)), descriptor((2, 9), torch.float32), descriptor((4, 8)), descriptor((4, 8)), None, None,
-                 0, None), "partial sums"),
-    (lambda f: f(descriptor((4, 8)), None, descriptor((4, 8)), descriptor((5, 8)), None, None, 0, None), "size mismatch"),
-])
-def test_activation_backward_refusals(call, match):
-    assert call(N.lib().tp_b200_activation_backward) < 0
-    assert match in N.lib().tp_b200_last_error().decode()
+def test_checkpoint_operands():
+    assert "null operand" in refused("tp_b200_checkpoint_pack", N.CHECKPOINT, CHECKPOINT, x=0)
+    assert "null operand" in refused("tp_b200_checkpoint_unpack", N.CHECKPOINT, CHECKPOINT, y=0)
+    assert "null operand" in refused("tp_b200_checkpoint_backward", N.CHECKPOINT, CHECKPOINT, x=0)
+    assert "null operand" in refused("tp_b200_checkpoint_backward", N.CHECKPOINT, CHECKPOINT, y=0)
+    for entry in ("pack", "unpack", "backward"):
+        call = getattr(N.lib(), f"tp_b200_checkpoint_{entry}")
+        assert call(N.CHECKPOINT.pack(*{**CHECKPOINT, "rows": 0}.values()), None) == 0
+        assert call(N.CHECKPOINT.pack(*{**CHECKPOINT, "n": 0, "values": 0}.values()), None) == 0
 
 
 def test_packed_arguments_match_the_header(tmp_path):
     """The structs Python packs have the sizes and offsets the C compiler gives them."""
     text = open(os.path.join(ROOT, "include", "tpb200.h")).read()
     lines = ['#include "tpb200.h"', "#include <stddef.h>", "#include <stdio.h>", "int main(void) {"]
-    for name in ("tpb_layer", "tpb_layer_grad", "tpb_tensor"):
+    for name in ("tpb_layer", "tpb_layer_grad", "tpb_checkpoint"):
         lines.append(f'printf("%zu\\n", sizeof({name}));')
-    last = {"tpb_layer": "w_work", "tpb_layer_grad": "w_work"}
+    last = {"tpb_layer": "w_work", "tpb_layer_grad": "w_work", "tpb_checkpoint": "exponents"}
     for name, field in last.items():
         lines.append(f'printf("%zu\\n", offsetof({name}, {field}));')
     source = tmp_path / "sizes.c"
@@ -128,14 +109,14 @@ def test_packed_arguments_match_the_header(tmp_path):
     binary = tmp_path / "sizes"
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(source), "-o", str(binary)], check=True)
     got = [int(v) for v in subprocess.run([str(binary)], check=True, capture_output=True, text=True).stdout.split()]
-    assert got[:3] == [N.LAYER.size, N.LAYER_GRAD.size, ctypes.sizeof(N.TpbTensor)]
-    assert got[3:] == [N.LAYER.size - 8, N.LAYER_GRAD.size - 8]
+    assert got[:3] == [N.LAYER.size, N.LAYER_GRAD.size, N.CHECKPOINT.size]
+    assert got[3:] == [N.LAYER.size - 8, N.LAYER_GRAD.size - 8, N.CHECKPOINT.size - 8]
     # field order: as many fields as values packed
-    for struct_name, packer in (("tpb_layer", N.LAYER), ("tpb_layer_grad", N.LAYER_GRAD)):
+    for struct_name, packer in (("tpb_layer", N.LAYER), ("tpb_layer_grad", N.LAYER_GRAD),
+                                ("tpb_checkpoint", N.CHECKPOINT)):
         body = re.search(r"typedef struct %s \{(.*?)\}" % struct_name, text, re.S).group(1)
         fields = sum(len(line.split(",")) for line in body.split(";") if line.strip())
         assert fields == len(packer.unpack(bytes(packer.size)))
-    assert struct.calcsize("Pii16q") == ctypes.sizeof(N.TpbTensor)
 
 
 def test_operators_refuse_host_tensors():
