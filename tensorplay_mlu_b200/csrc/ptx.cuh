@@ -103,6 +103,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// Fetch a tensor-map box into L2 only.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1)
+                 : "memory");
+}
+
 // The same loads for a CTA pair (cta_group::2): the bytes land in this CTA's
 // shared memory and complete_tx is signalled on the barrier at `bar`, a
 // shared::cluster address (the pair leader's barrier).  No multicast.
