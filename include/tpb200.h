@@ -461,12 +461,13 @@ typedef struct tpb_layer {
 int tp_b200_layer_forward(const tpb_layer* layer, void* stream);
 
 /* Its gradients: dz = dy act'(z), or [dy zu act'(zg) | dy act(zg)] for the
- * gated block, from dy and what was saved -- either `saved`, contiguous, or values and exponents; neither is
- * needed or read for parts 1 without an activation -- and from it
- * dx [m, k] = dz w, dw [parts * n, k] = dz^T x (both contiguous), db [parts *
- * n] = the column sums of dz before its rounding.  dx, dw, db may be NULL.
- * dz: workspace [m, parts * n], row stride dz_stride; partial: workspace of
- * groups * parts * n floats when db is wanted (1 <= groups <= 65535 groups of
+ * gated block, from dy and what was saved -- either `saved`, contiguous, or
+ * values and exponents; neither is needed or read for parts 1 without an
+ * activation -- and from it dx [m, k] = dz w, dw [parts * n, k] = dz^T x (both
+ * contiguous), db [parts * n] = the column sums of dz before its rounding to
+ * the layer's dtype (float16: beyond 65504 it is infinite).  dx, dw, db may be
+ * NULL.  dz: workspace [m, parts * n], row stride dz_stride; partial: workspace
+ * of groups * parts * n floats when db is wanted (1 <= groups <= 65535 groups of
  * rows are summed apart, then joined in order); x_work, w_work as above. */
 typedef struct tpb_layer_grad {
     int32_t dtype, act, parts, flags;

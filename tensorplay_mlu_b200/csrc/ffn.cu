@@ -351,6 +351,13 @@ __host__ __device__ constexpr int backward_blocks() {
 // the fp32 sums of dz (before its rounding) over the block's rows.  A thread
 // keeps its V columns and walks the rows, so the sums stay in registers; they
 // are joined over the block in a fixed order and written as one partial row.
+// dz is computed in fp32 and rounded once, to T: the two products want operands
+// of T (a 16-bit MMA has nominally six times the rate of three TF32 ones, and
+// dz is written once and read twice).  That rounding is half a step of each
+// element, as large as the results' own, so dx and dw are off by about sqrt(2)
+// times the final rounding alone.  In float16 an element of dz beyond 65504 is
+// infinite and one below 6e-5 loses bits, as with separate float16 layers:
+// gradients are scaled as for those.
 template <typename T, int V, bool GATED, bool SAVED8, int MODE, bool SUMS>
 __global__ void __launch_bounds__(kThreads, (backward_blocks<T, GATED>())) ffn_backward_kernel(const BackwardParams<T> p) {
     pdl_entry();

@@ -3,11 +3,16 @@
 //
 // Every operand element is split on its way into shared memory, x = hi + lo
 // with hi = x rounded to TF32 and lo = x - hi, read by the MMA as TF32 too, and
-// a product is hi hi + hi lo + lo hi: three TF32 MMAs.  The dropped lo lo and
-// lo's lost bits are at most 2^-21 of |a b|.  The tensor core rounds its running sum towards
-// zero, so a TMEM accumulator only takes kChain k-blocks (kChain * 32 terms);
-// warps of their own then add it to fp32 sums in registers, rounded to
-// nearest, while the MMAs fill the other accumulator.
+// a product is hi hi + hi lo + lo hi: three TF32 MMAs, the last two into an
+// accumulator of their own.  The dropped lo lo and lo's lost bits are at most
+// 2^-21 of |a b|.  The tensor core rounds its running sum towards zero, so a
+// TMEM accumulator only takes kChain k-blocks (kChain * 32 terms); warps of
+// their own then add it to fp32 sums in registers, rounded to nearest, while
+// the MMAs fill the other accumulator.
+//
+// What bounds it: the loader warps' instructions (2048 x 4096 -> 4096: 722 us,
+// 95 TFLOP/s, tensor pipe 26 %).  Sixteen loader warps on narrower tiles, and
+// persistent CTAs, measured slower.
 //
 // Why not pre-split copies and library-style tiles: those write and read each
 // operand three times and take a launch per chunk of K; for the sizes of a

@@ -1292,7 +1292,9 @@ def gated_linear(input, weight, bias=None, activation: str = "silu"):
 def native_gated_linear_backward(grad_output, input, weight, saved, activation: str = "silu",
                                  output_mask=(True, True, True)):
     """(dinput, dweight, dbias) of :func:`native_gated_linear`, each None where ``output_mask`` says so.
-    ``saved`` is what the forward pass returned."""
+    ``saved`` is what the forward pass returned.  The pre-activations' gradient
+    is held in the input's dtype between its kernel and the two products, as
+    between separate layers (in float16 with float16's range)."""
     return _layer_backward("native_gated_linear_backward", grad_output, input, weight, saved, activation, 2,
                            output_mask)
 
