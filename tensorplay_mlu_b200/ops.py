@@ -1140,7 +1140,7 @@ def checkpoint_pack(x):
 
 def checkpoint_unpack(values, exponents, dtype: torch.dtype):
     """The tensor an 8-bit checkpoint stands for, in ``dtype`` (exact in
-    bfloat16 and float32; float16 underflows below its subnormals)."""
+    bfloat16 and float32, rounded to float16 within its range)."""
     _require_device(values)
     if dtype not in _FFN_DTYPES:
         raise RuntimeError(f"checkpoint_unpack: expected bfloat16, float16 or float32, got {dtype}")
