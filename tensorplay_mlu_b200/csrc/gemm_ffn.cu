@@ -144,13 +144,20 @@ __device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUten
                 }
             }
             if (kParts == 2) __syncwarp();
-        } else if (f.values != nullptr) {
+        }
+        if (f.values != nullptr) {
+            if (f.saved != nullptr) {
+                // Both forms are kept: the second tile once more, when z has
+                // left it.
+                if (lane == 0) bulk_wait_group_read0();
+                __syncwarp();
+            }
 #pragma unroll
             for (int q = 0; q < kParts; ++q) {
                 const uint8_t stored = stage_checkpoint<T>(stage2 + q * 1024, lane, z[q]);
                 if (lane < rows) f.exponents[((row0 + lane) * kParts + q) * f.nb + (n >> 5)] = stored;
             }
-            if (!f.saved_tma) {
+            if (!f.values_tma) {
                 __syncwarp();
 #pragma unroll
                 for (int q = 0; q < kParts; ++q) {
@@ -190,7 +197,7 @@ __device__ void store_ffn(const TcParams& p, const CUtensorMap* tmC, const CUten
         __syncwarp();
         if (lane == 0) {
             if (p.tma_store) tma_store_2d(tmC, smem_addr(stage), int(n), int(row0));
-            if (f.values != nullptr && f.saved_tma) {
+            if (f.values_tma) {
 #pragma unroll
                 for (int q = 0; q < kParts; ++q) {
                     tma_store_3d(tmSaved, smem_addr(stage2 + q * 1024), int(n), q, int(row0));
@@ -253,11 +260,14 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
         f.ssaved_p = q.N;
         f.saved_tma = aligned16(q.saved) && (q.N * es) % 16 == 0;
         if (f.saved_tma) ms = make_saved_map(q.saved, type, es, q.N, q.parts, q.M, f.ssaved_p, f.ssaved_m);
-    } else if (q.values != nullptr) {
+    }
+    if (q.values != nullptr) {
         f.values = q.values;
         f.exponents = q.exponents;
-        f.saved_tma = aligned16(q.values) && q.N % 16 == 0;
-        if (f.saved_tma) {
+        // One tensor map serves both forms; asked for together, the bytes go
+        // out by ordinary stores.
+        f.values_tma = q.saved == nullptr && aligned16(q.values) && q.N % 16 == 0;
+        if (f.values_tma) {
             ms = make_saved_map(q.values, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.N, q.parts, q.M, q.N, q.parts * q.N);
         }
     }

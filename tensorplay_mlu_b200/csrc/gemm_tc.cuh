@@ -150,7 +150,8 @@ struct FfnParams {
     int64_t nb;            // checkpoint blocks of a row
     int act;
     int residual_vec;      // residual rows on 16-byte boundaries
-    int saved_tma;         // saved / values are written by TMA stores
+    int saved_tma;         // saved is written by TMA stores
+    int values_tma;        // values are (only one of the two: a map for both)
 };
 
 struct TcParams {
