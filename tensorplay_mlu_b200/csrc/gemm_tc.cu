@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                           half * (BN / 2), b, gm, gm - lane, int64_t(nt) * BN,
                                                           gm < p.M);
             } else {
-                store_accumulator<T, BN / 2>(p, staging + (warp - 2) * staging_bytes<T>(), t_rows, half * (BN / 2), b,
-                                             gm, int64_t(nt) * BN, gm < p.M);
+                store_accumulator_plain<T, BN / 2>(p, staging + (warp - 2) * staging_bytes<T>(), t_rows, half * (BN / 2),
+                                                   b, gm, int64_t(nt) * BN, gm < p.M);
             }
             tc_fence_before();
             __syncwarp();
