@@ -27,6 +27,10 @@
 // step of the largest float round to inf, so such a sum comes out NaN; every
 // NaN sum is recomputed as a plain fp32 dot product, which gives the infinity
 // or NaN that fp32 arithmetic gives.
+//
+// Where the caller allows one TF32 product (ONCE, kernels of their own) only
+// hi hi is computed, and lo is neither made nor stored.  There a rounding past
+// the range shows as an infinity, so sums that are infinite are recomputed too.
 
 #include "gemm_few.cuh"
 
@@ -42,7 +46,6 @@ struct F32Operands {
     const float* x;  // element (m, k) at x + m * sx_m + k * sx_k
     int64_t sx_m, sx_k;
     int vec_w, vec_x;  // 16-byte loads along the unit stride
-    int tf32;          // one TF32 product is enough
 };
 
 template <int NT>
@@ -67,12 +70,27 @@ __device__ __forceinline__ float4 ldg128(const float* p) {
     return v;
 }
 
+// x for a single TF32 product: rounded to nearest, ties away.  An infinity stays
+// one, and a NaN one, whatever its payload (the addition below would carry
+// 0x7fffffff into a zero); a finite x past the largest TF32 becomes an infinity.
+__device__ __forceinline__ float tf32_once(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return __uint_as_float(r);
+}
+
 // hi and lo of four consecutive k (chunk q) of row r into their swizzled
 // tiles.  hi is rounded to nearest, ties away; lo's low bits are the MMA's to
-// drop (2^-10 of lo).  An infinity keeps hi = inf and makes lo NaN, a NaN
-// makes lo NaN.
+// drop (2^-10 of lo).  An infinity keeps hi = inf and makes lo NaN; a NaN makes
+// lo NaN, whatever the addition leaves of it in hi (0x7fffffff: a zero).
+// ONCE: hi alone, which then has to keep them itself.
+template <bool ONCE>
 __device__ __forceinline__ void store_split(uint8_t* hi_tile, uint32_t lo_offset, int r, int q, float4 v) {
     uint8_t* at = hi_tile + r * 128 + ((q ^ (r & 7)) << 4);
+    if constexpr (ONCE) {
+        *reinterpret_cast<float4*>(at) = make_float4(tf32_once(v.x), tf32_once(v.y), tf32_once(v.z), tf32_once(v.w));
+        return;
+    }
     const auto hi = [](float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); };
     const float4 h = make_float4(hi(v.x), hi(v.y), hi(v.z), hi(v.w));
     *reinterpret_cast<float4*>(at) = h;
@@ -83,7 +101,7 @@ __device__ __forceinline__ void store_split(uint8_t* hi_tile, uint32_t lo_offset
 // Along k (MN false): chunk q of rows r0 + 32 i, eight lanes a row.  Along the
 // rows (MN true): rows r0 .. r0 + 3 at four k, transposed by the store; the
 // lanes are numbered so that eight neighbours store to distinct banks.
-template <bool MN, int kRows>
+template <bool MN, int kRows, bool ONCE>
 struct Loader {
     static constexpr int kRegs = MN ? 4 : kRows / 32;
     const float* ptr[MN ? 1 : kRegs];
@@ -164,24 +182,24 @@ struct Loader {
     __device__ __forceinline__ void store(uint8_t* tile, uint32_t lo_offset, const float4 (&reg)[kRegs]) const {
         if constexpr (MN) {
             if (!active) return;
-            store_split(tile, lo_offset, r0, q, make_float4(reg[0].x, reg[1].x, reg[2].x, reg[3].x));
-            store_split(tile, lo_offset, r0 + 1, q, make_float4(reg[0].y, reg[1].y, reg[2].y, reg[3].y));
-            store_split(tile, lo_offset, r0 + 2, q, make_float4(reg[0].z, reg[1].z, reg[2].z, reg[3].z));
-            store_split(tile, lo_offset, r0 + 3, q, make_float4(reg[0].w, reg[1].w, reg[2].w, reg[3].w));
+            store_split<ONCE>(tile, lo_offset, r0, q, make_float4(reg[0].x, reg[1].x, reg[2].x, reg[3].x));
+            store_split<ONCE>(tile, lo_offset, r0 + 1, q, make_float4(reg[0].y, reg[1].y, reg[2].y, reg[3].y));
+            store_split<ONCE>(tile, lo_offset, r0 + 2, q, make_float4(reg[0].z, reg[1].z, reg[2].z, reg[3].z));
+            store_split<ONCE>(tile, lo_offset, r0 + 3, q, make_float4(reg[0].w, reg[1].w, reg[2].w, reg[3].w));
         } else {
 #pragma unroll
-            for (int i = 0; i < kRegs; ++i) store_split(tile, lo_offset, r0 + 32 * i, q, reg[i]);
+            for (int i = 0; i < kRegs; ++i) store_split<ONCE>(tile, lo_offset, r0 + 32 * i, q, reg[i]);
         }
     }
 };
 
-template <int PARTS, int NT, bool W_MN, bool X_MN>
+template <int PARTS, int NT, bool W_MN, bool X_MN, bool ONCE>
 __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(const FewParams p, const F32Operands o) {
     using S = F32Shape<NT>;
     constexpr int kStages = S::kStages;
     constexpr int kColumns = 128 / PARTS;
-    using LoadW = Loader<W_MN, 128>;
-    using LoadX = Loader<X_MN, NT>;
+    using LoadW = Loader<W_MN, 128, ONCE>;
+    using LoadX = Loader<X_MN, NT, ONCE>;
     constexpr int kDepth = LoadW::kRegs + LoadX::kRegs > 6 ? 2 : 3;  // k-blocks in registers
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -296,7 +314,7 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
                 const uint64_t x_hi = w_lo + S::kWBytes / 16;  // x_lo behind it
                 const uint32_t d = tmem + acc * 2 * NT;
                 uint32_t more = i % kChain != 0 ? 1u : 0u;
-                if (o.tf32) {
+                if constexpr (ONCE) {
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         umma<true>(d, w_hi + kk * 2, x_hi + kk * 2, p.idesc, more);
@@ -343,7 +361,7 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
 #pragma unroll
             for (int c = 0; c < S::kAccCols; c += 16) {
                 uint32_t r[16];
-                if (!o.tf32) {
+                if constexpr (!ONCE) {
                     tmem_ld16(at + NT + c, r);
                     tmem_wait_ld();
 #pragma unroll
@@ -369,11 +387,12 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // every CTA's partial sums are in its shared memory
-    // A NaN sum is computed again as fp32 arithmetic would.
+    // A NaN sum (ONCE: or an infinite one) is computed again as fp32 arithmetic
+    // would.
     finish_rows<float, PARTS, NT>(
         p, reinterpret_cast<const float*>(smem), m0, n0, warp, S::kThreads / 32, rank, ranks,
         [&](int64_t m, int64_t n, int q, float& z) {
-            if (z == z || n >= p.N) return;
+            if ((ONCE ? fabsf(z) < INFINITY : z == z) || n >= p.N) return;
             const float* w = o.w + (n + int64_t(q) * p.N) * o.sw_n;
             const float* x = o.x + m * o.sx_m;
             z = 0.0f;
@@ -387,11 +406,11 @@ __global__ void __launch_bounds__(F32Shape<NT>::kThreads, 1) gemm_f32_kernel(con
     }
 }
 
-template <int PARTS, int NT, bool W_MN, bool X_MN>
+template <int PARTS, int NT, bool W_MN, bool X_MN, bool ONCE>
 void launch_f32(FewParams& p, const F32Operands& o, int dev, cudaStream_t stream) {
     using S = F32Shape<NT>;
-    auto kern = gemm_f32_kernel<PARTS, NT, W_MN, X_MN>;
-    const Slots& slots = cluster_slots<gemm_f32_kernel<PARTS, NT, W_MN, X_MN>>(S::kThreads, S::kSmem, dev);
+    auto kern = gemm_f32_kernel<PARTS, NT, W_MN, X_MN, ONCE>;
+    const Slots& slots = cluster_slots<gemm_f32_kernel<PARTS, NT, W_MN, X_MN, ONCE>>(S::kThreads, S::kSmem, dev);
     p.idesc = (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(NT >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     p.row_tiles = (p.M + NT - 1) / NT;
     const int64_t tiles = int64_t(p.row_tiles) * ((p.N + 128 / PARTS - 1) / (128 / PARTS));
@@ -400,13 +419,19 @@ void launch_f32(FewParams& p, const F32Operands& o, int dev, cudaStream_t stream
     check_launch("gemm_f32");
 }
 
-template <int PARTS, bool W_MN, bool X_MN>
+template <int PARTS, bool W_MN, bool X_MN, bool ONCE>
 void launch_rows(FewParams& p, const F32Operands& o, int dev, cudaStream_t stream) {
     // 128 rows a tile where that still gives every SM one, fewer otherwise.
     const int64_t columns = (p.N + 128 / PARTS - 1) / (128 / PARTS);
-    if (p.M <= 32) launch_f32<PARTS, 32, W_MN, X_MN>(p, o, dev, stream);
-    else if (p.M <= 64 || columns * ((p.M + 127) / 128) < num_sms(dev)) launch_f32<PARTS, 64, W_MN, X_MN>(p, o, dev, stream);
-    else launch_f32<PARTS, 128, W_MN, X_MN>(p, o, dev, stream);
+    if (p.M <= 32) launch_f32<PARTS, 32, W_MN, X_MN, ONCE>(p, o, dev, stream);
+    else if (p.M <= 64 || columns * ((p.M + 127) / 128) < num_sms(dev)) launch_f32<PARTS, 64, W_MN, X_MN, ONCE>(p, o, dev, stream);
+    else launch_f32<PARTS, 128, W_MN, X_MN, ONCE>(p, o, dev, stream);
+}
+
+template <int PARTS, bool W_MN, bool X_MN>
+void launch_products(bool once, FewParams& p, const F32Operands& o, int dev, cudaStream_t stream) {
+    if (once) launch_rows<PARTS, W_MN, X_MN, true>(p, o, dev, stream);
+    else launch_rows<PARTS, W_MN, X_MN, false>(p, o, dev, stream);
 }
 
 // 16-byte loads: along k rows have to start on such boundaries, along the rows
@@ -424,16 +449,16 @@ void gemm_f32(const FfnProblem& q, int dev, cudaStream_t stream) {
     o.x = static_cast<const float*>(q.x);
     o.sx_m = q.sx_m;
     o.sx_k = q.sx_k;
-    o.tf32 = (q.flags & TPB_GEMM_ALLOW_TF32) != 0;
+    const bool once = (q.flags & TPB_GEMM_ALLOW_TF32) != 0;  // one TF32 product is enough
     // A layer reads w and x along k; dz w reads w along its rows' elements,
     // dz^T x both operands (w's strides are then both 1 when it has one column).
     const bool x_mn = q.sx_k != 1, w_mn = q.sw_k != 1 || x_mn;
     o.vec_w = vectors(o.w, w_mn ? o.sw_k : o.sw_n);
     o.vec_x = vectors(o.x, x_mn ? o.sx_k : o.sx_m);
-    if (q.parts == 2) launch_rows<2, false, false>(p, o, dev, stream);
-    else if (!w_mn) launch_rows<1, false, false>(p, o, dev, stream);
-    else if (!x_mn) launch_rows<1, true, false>(p, o, dev, stream);
-    else launch_rows<1, true, true>(p, o, dev, stream);
+    if (q.parts == 2) launch_products<2, false, false>(once, p, o, dev, stream);
+    else if (!w_mn) launch_products<1, false, false>(once, p, o, dev, stream);
+    else if (!x_mn) launch_products<1, true, false>(once, p, o, dev, stream);
+    else launch_products<1, true, true>(once, p, o, dev, stream);
 }
 
 }  // namespace tpb
