@@ -637,6 +637,9 @@ void require_layer(int dtype, int act, int parts, int64_t m, int64_t n, int64_t 
     const int64_t limit = int64_t(1) << 30;
     TPB_CHECK(m >= 0 && n >= 0 && k >= 0 && m < limit && n < limit && k < limit,
               "%s: sizes %lld, %lld, %lld out of range", what, (long long)m, (long long)n, (long long)k);
+    // The products count rows and columns in 32 bits, a tile of 256 past the end
+    // included; the gradients' contract over, and have rows for, both parts.
+    TPB_CHECK(parts * n <= INT32_MAX - 256, "%s: %lld rows of the weight are out of range", what, (long long)(parts * n));
 }
 
 // A checkpoint entry point: its checks, then body(T{}, device, stream).

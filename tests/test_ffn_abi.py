@@ -128,3 +128,11 @@ def test_operators_refuse_host_tensors():
             call()
     with pytest.raises(RuntimeError, match="activation must be one of"):
         ops.gated_linear(x, w, None, "swish")
+
+
+@pytest.mark.parametrize("n", [(1 << 30) - 1, (1 << 30) - 128])
+def test_weight_rows_whose_tiles_pass_32_bits_are_refused(n):
+    """Both parts together are a dimension of the gradients' products, which
+    count it, and the last tile's rows, in 32-bit integers."""
+    assert "out of range" in refused("tp_b200_layer_forward", N.LAYER, LAYER, n=n, y_stride=n)
+    assert "out of range" in refused("tp_b200_layer_backward", N.LAYER_GRAD, GRAD, n=n, dy_stride=n, dz_stride=2 * n)
