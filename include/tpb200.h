@@ -105,7 +105,9 @@ int64_t tp_b200_launch_count(void);
  * lowers it around a GEMM that overlaps a collective, so the collective's
  * kernels find free SMs instead of delaying the GEMM's statically
  * scheduled tiles.  Process-wide per device; affects launches, not
- * kernels already queued. */
+ * kernels already queued.  Feed-forward layers keep to it in bfloat16 and
+ * float16 beyond 64 rows; up to 64 rows, and in float32, their products are
+ * not persistent and run on any SM that is free. */
 int tp_b200_set_gemm_sm_limit(int dev, int sms);
 /* Tile order of the CTA-pair tensor-core GEMMs launched afterwards on `dev`:
  * 0 (default) a fixed order (tile c + i * clusters to cluster c); non-zero

@@ -283,12 +283,15 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
 // 4096 -> 512: 27 / 9; 384 x 4096 -> 2048: 28 / 23; 576 x 1024 -> 2048: 12.6 /
 // 11.3; 1024 x 1024 -> 2048: 12.7 / 13.6; 2048 x 4096 -> 6000: 79 / 108.  The
 // estimate here: 0.31 us for each 64-deep step of a wave of 256 x 256 tiles,
-// 2.2 us for a wave's ramp and epilogue, 5 us once.
+// 2.2 us for a wave's ramp and epilogue, 5 us once.  Under an SM limit
+// (tp_b200_set_gemm_sm_limit) only this kernel, which is persistent, leaves the
+// other SMs alone.
 bool few_rows(const FfnProblem& q, int dev) {
     if (q.M <= 64 && q.sx_k == 1) return true;
+    if (gemm_sm_budget(dev) < num_sms(dev)) return false;
     const int64_t columns = q.parts == 2 ? 128 : kPairBN;
     const int64_t tiles = ((q.M + kPairBM - 1) / kPairBM) * ((q.N + columns - 1) / columns);
-    const int64_t clusters = std::max(1, gemm_sm_budget(dev) / 2);
+    const int64_t clusters = std::max(1, num_sms(dev) / 2);
     const double waves = static_cast<double>((tiles + clusters - 1) / clusters);
     return gemm_few_us(q, dev) < 5.0 + waves * (0.3125 * static_cast<double>((q.K + 63) / 64) + 2.2);
 }
