@@ -1025,7 +1025,8 @@ def layer_norm(input, normalized_shape, weight=None, bias=None, eps: float = 1e-
 # The gated feed-forward block, a linear layer with its activation and the
 # residual stream, and 8-bit checkpoints of what their backward passes need.
 # Not among the reference's registrations (there they are sequences of linear,
-# an activation, mul and add), so they stand outside KERNELS.
+# an activation, mul and add), so they stand outside KERNELS; FEED_FORWARD
+# lists them for the profiler.
 
 _FFN_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _BLOCK = N.CHECKPOINT_BLOCK
@@ -1321,6 +1322,10 @@ def native_linear_act_backward(grad_output, input, weight, saved, activation: st
     not read and may be None."""
     return _layer_backward("native_linear_act_backward", grad_output, input, weight, saved, activation, 1,
                            output_mask)
+
+
+FEED_FORWARD = (checkpoint_pack, checkpoint_unpack, checkpoint_activation_backward, native_gated_linear, gated_linear,
+                native_gated_linear_backward, native_linear_act, linear_act, native_linear_act_backward)
 
 
 # -------------------------------------------------------------------- index

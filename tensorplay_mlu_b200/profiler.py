@@ -5,9 +5,10 @@ around every operation (``current_device``, ``record``, ``elapsed_ms``,
 ``release``), over pooled CUDA timing events recorded on the device's current
 stream (``tp_b200_timer_*``).  ``profile`` is the same measurement for this
 package's operator functions when TensorPlay's profiler is not there: inside
-the ``with`` block every registered operator (``ops.KERNELS``) is bracketed
-by two records, and ``key_averages()`` reports per operator the call count,
-device time and host time, like ``profile(activities=[PrivateUse1])``.
+the ``with`` block every registered operator (``ops.KERNELS``) and every
+feed-forward one (``ops.FEED_FORWARD``) is bracketed by two records, and
+``key_averages()`` reports per operator the call count, device time and host
+time, like ``profile(activities=[PrivateUse1])``.
 
     with profile() as prof:
         for _ in range(3):
@@ -98,7 +99,7 @@ def _key(schema: str) -> str:
 
 @dataclass
 class profile:
-    """Time every registered operator called inside the block on the device."""
+    """Time every operator called inside the block on the device."""
 
     activities: list = field(default_factory=lambda: [ProfilerActivity.CPU, ProfilerActivity.PrivateUse1])
 
@@ -116,6 +117,7 @@ class profile:
         by_function = {}
         for schema, fn in ops.KERNELS.items():
             by_function.setdefault(id(fn), _key(schema))
+        by_function.update({id(fn): fn.__name__ for fn in ops.FEED_FORWARD})
         timed = ProfilerActivity.PrivateUse1 in self.activities
         lib = N.lib()
         for name in dir(ops):
