@@ -411,9 +411,14 @@ int tp_b200_gemm_epilogue(int epilogue, const tpb_tensor* out, const tpb_tensor*
  * block of 32 consecutive elements of a row is int8 values q and one uint8
  * exponent s, standing for q * 2^(s - 127): the least power of two with
  * max|x| <= 127 * 2^(s - 127), x / 2^(s - 127) rounded to the nearest
- * integer, ties to even.  s = 255 marks a block that held an infinity or a
- * NaN and reads back as NaN.  values has the tensor's shape, exponents
- * ceil(n / 32) in the last dimension; both contiguous.
+ * integer, ties to even: off by at most half of 2^(s - 127).  At the ends of
+ * the range: in a block whose largest magnitude would round to 64 * 2^(s - 127)
+ * past the dtype's largest value (float16: from 65024 up; bfloat16 and float32:
+ * from 127 * 2^121 up), q stops at 63 in magnitude and is off by less than
+ * 2^(s - 127); and s is at least 1, so magnitudes up to 2^-127 read back as
+ * zero.  s = 255 marks a block that held an infinity or a NaN and reads back as
+ * NaN.  values has the tensor's shape, exponents ceil(n / 32) in the last
+ * dimension; both contiguous.
  * ---------------------------------------------------------------------- */
 
 enum tpb_activation {

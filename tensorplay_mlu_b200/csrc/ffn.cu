@@ -1,6 +1,7 @@
-// Elementwise kernels of the feed-forward operators: the activation, gate and
-// residual behind a product (where the product's own epilogue does not apply
-// them), their backward pass with the bias gradient, and 8-bit checkpoints.
+// Elementwise kernels of the feed-forward operators: the gradients of
+// activation and gate with the bias gradient, 8-bit checkpoints, and the
+// activation, gate and residual of a layer without input features (others
+// have them in their product's epilogue).
 //
 // tensorplay-mlu runs these as separate activation, mul and add kernels
 // (UnaryKernels.cpp:52-104, BinaryKernels.cpp:148-248) and has no
@@ -690,7 +691,8 @@ Aligned align_rows(const void* src, int64_t pitch, int64_t rows, int64_t n, int 
     return {work, aligned};
 }
 
-// x w^T without an epilogue, for the plain products' kernels.
+// x w^T without an epilogue, for the plain products' kernels: gradients with a
+// dimension of 2^30 or more, which the feed-forward products leave.
 GemmProblem plain_product(const FfnProblem& q) {
     GemmProblem g{};
     g.dtype = q.dtype;

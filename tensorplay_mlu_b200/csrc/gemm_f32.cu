@@ -10,13 +10,15 @@
 // their own then add it to fp32 sums in registers, rounded to nearest, while
 // the MMAs fill the other accumulator.
 //
-// What bounds it: the loader warps' instructions (2048 x 4096 -> 4096: 722 us,
-// 95 TFLOP/s, tensor pipe 26 %).  Sixteen loader warps on narrower tiles, and
-// persistent CTAs, measured slower.
+// What bounds it: the loader warps' instructions (2048 x 4096 -> 4096: 745 us,
+// 92 TFLOP/s, tensor pipe 26 %), among them spills of the 128-row tiles: 17
+// warps leave 96 registers a thread, and a K-major tile stores 132 and loads
+// 188 bytes of them.  Sixteen loader warps on narrower tiles, and persistent
+// CTAs, measured slower.
 //
-// Why not pre-split copies and library-style tiles: those write and read each
-// operand three times and take a launch per chunk of K; for the sizes of a
-// layer (512 x 1024 x 4096) the launches alone cost more than the product.
+// Why not the plain product's pre-split copies: those write and read each
+// operand three times and take a launch per 1024 of K, and have no epilogue.
+// They win where the product is large, 4096^3: 1.03 ms against 1.44 here.
 //
 // Operands are read with plain loads (any strides, no alignment needed: a
 // transposed operand is read along its unit stride and transposed by the

@@ -27,7 +27,6 @@ struct FewParams {
     int M, N, K;       // rows of x; result columns of one part; contraction
     int k_blocks;
     int row_tiles;     // ceil(M / kNT)
-    int tiles;         // gemm_f32.cu: tiles of the whole product
     uint32_t idesc;
     void* y;
     int64_t sy_m;

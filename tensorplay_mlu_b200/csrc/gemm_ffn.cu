@@ -281,8 +281,11 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
 // always (its bound is the weight's one reading), beyond where its estimated
 // time is below this kernel's.  Measured, bf16, us, pair / split: 100 rows x
 // 4096 -> 512: 27 / 9; 384 x 4096 -> 2048: 28 / 23; 576 x 1024 -> 2048: 12.6 /
-// 11.3; 1024 x 1024 -> 2048: 12.7 / 13.6; 2048 x 4096 -> 6000: 79 / 108.  The
-// estimate here: 0.31 us for each 64-deep step of a wave of 256 x 256 tiles,
+// 11.3; 1024 x 1024 -> 2048: 12.7 / 13.6; 2048 x 4096 -> 6000: 79 / 108; dz^T x
+// of 13898 rows, 304 x 120: 77 / 16.  The estimates were fitted to forward
+// products that keep nothing, and are worst where the split kernel's epilogue
+// stores 8 bits (gated, 300 x 2048 -> 2 * 2048: 19 / 32, the slower one taken)
+// and in dz w (512 x 4096 -> 4096: 27 / 32, the same).  The estimate here: 0.31 us for each 64-deep step of a wave of 256 x 256 tiles,
 // 2.2 us for a wave's ramp and epilogue, 5 us once.  Under an SM limit
 // (tp_b200_set_gemm_sm_limit) only this kernel, which is persistent, leaves the
 // other SMs alone.

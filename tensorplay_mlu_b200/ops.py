@@ -1122,8 +1122,11 @@ def checkpoint_pack(x):
     two: ``values`` (int8, x's shape) times ``2 ** (exponents - 127)``
     (uint8, one per block), the least power for which the block fits, each
     value rounded to nearest, ties to even.  The error is at most half that
-    power of two, 1/127 of the block's largest magnitude at worst.  A block
-    that holds an infinity or a NaN reads back as NaN."""
+    power of two, 1/127 of the block's largest magnitude at worst; but up to the
+    whole of it in a block whose largest magnitude, rounded, would leave the
+    dtype's range (float16: from 65024 up), where values stop at 63, and 2^-127
+    where the power is the smallest, 2^-126.  A block that holds an infinity or
+    a NaN reads back as NaN."""
     _ffn_check("checkpoint_pack", x)
     if x.dim() == 0:
         raise RuntimeError("checkpoint_pack: expected at least one dimension")
