@@ -426,7 +426,8 @@ void launch_rows(FewParams& p, const F32Operands& o, int dev, cudaStream_t strea
     // 128 rows a tile where that still gives every SM one, fewer otherwise.
     const int64_t columns = (p.N + 128 / PARTS - 1) / (128 / PARTS);
     if (p.M <= 32) launch_f32<PARTS, 32, W_MN, X_MN, ONCE>(p, o, dev, stream);
-    else if (p.M <= 64 || columns * ((p.M + 127) / 128) < num_sms(dev)) launch_f32<PARTS, 64, W_MN, X_MN, ONCE>(p, o, dev, stream);
+    else if (p.M <= 64 || columns * ((p.M + 127) / 128) < num_sms(dev))
+        launch_f32<PARTS, 64, W_MN, X_MN, ONCE>(p, o, dev, stream);
     else launch_f32<PARTS, 128, W_MN, X_MN, ONCE>(p, o, dev, stream);
 }
 

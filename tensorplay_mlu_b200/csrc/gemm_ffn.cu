@@ -285,10 +285,10 @@ void launch_ffn_pair(const FfnProblem& q, int dev, cudaStream_t stream, CUtensor
 // of 13898 rows, 304 x 120: 77 / 16.  The estimates were fitted to forward
 // products that keep nothing, and are worst where the split kernel's epilogue
 // stores 8 bits (gated, 300 x 2048 -> 2 * 2048: 19 / 32, the slower one taken)
-// and in dz w (512 x 4096 -> 4096: 27 / 32, the same).  The estimate here: 0.31 us for each 64-deep step of a wave of 256 x 256 tiles,
-// 2.2 us for a wave's ramp and epilogue, 5 us once.  Under an SM limit
-// (tp_b200_set_gemm_sm_limit) only this kernel, which is persistent, leaves the
-// other SMs alone.
+// and in dz w (512 x 4096 -> 4096: 27 / 32, the same).  The estimate here: 0.31
+// us for each 64-deep step of a wave of 256 x 256 tiles, 2.2 us for a wave's
+// ramp and epilogue, 5 us once.  Under an SM limit (tp_b200_set_gemm_sm_limit)
+// only this kernel, which is persistent, leaves the other SMs alone.
 bool few_rows(const FfnProblem& q, int dev) {
     if (q.M <= 64 && q.sx_k == 1) return true;
     if (gemm_sm_budget(dev) < num_sms(dev)) return false;

@@ -133,7 +133,7 @@ def test_infinities_and_the_largest_values(ops, m):
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.isinf(), want.isinf())
         assert torch.equal(got[want.isinf()].double(), want[want.isinf()])
-    # The largest floats would round past the range: they are cut to 11 bits instead, off by less than 2^-10.
+    # The largest floats round past the range: their sums are computed again in fp32, or cut to 11 bits (2^-10).
     top = torch.finfo(torch.float32).max
     big = torch.full((m, 4), top, device="cuda")
     big[:, 1] = -top
